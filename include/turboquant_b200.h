@@ -375,6 +375,30 @@ int tq_nc_decode_paged(const void* q, int q_dtype, int batch, int num_q_heads, i
                        void* out, int out_dtype, float* out_lse, int num_ctas, void* stream);
 int tq_nc_write_dropped(int32_t* count);
 
+/* ---------------------------------------------------------------------------------------
+ * Eviction by accumulated attention weight.  Of every sequence's len tokens, for each KV head, the last
+ * `recent` stay and of the others those of the largest scores, min(len, keep) in all; a tie goes to the lower
+ * position, a NaN counts as -inf.  What stays keeps its order and moves to positions 0, 1, ... : whole slots of K and V, in the pages of
+ * out_page_table, or (null) in the sequence's own pages.
+ *   page_table    int32 [batch][max_pages], seq_lens int32 [batch] (device)
+ *   scores        fp32, element [b * batch stride + h * head stride + position]; max_tokens: positions a row has
+ *   out_page_table int32 [batch][out_max_pages], at least min(keep, longest) tokens wide; its pages are none of those that the call reads
+ *   out_scores    fp32, the kept scores by their new position; may be `scores` itself
+ *   kept          int32 [batch][num_kv_heads][keep]: the position each kept token had, ascending, then -1
+ *   new_lens      int32 [batch]: min(len, keep)
+ * Slots, scores and pages behind the last kept token are left as they are.  A sequence of a negative length, or longer than its
+ * pages or scores, keeps nothing and is counted, as is a page id outside [0, num_blocks), whose rows are not moved (tq_state_fault_counts).
+ * block_size 16; any slot of a multiple of 4 bytes.  The workspace (tq_evict_workspace_bytes, max_tokens = the smaller of 16 max_pages and the scores'
+ * row) is needed where rows or scores stay in their place, 256-byte aligned, and needs no initialising.  The reference keeps every token. */
+size_t tq_evict_workspace_bytes(int batch, int num_kv_heads, int slot_bytes, int max_tokens, int keep, int in_place, int scores_in_place);
+int tq_evict(void* kv_cache, int64_t num_blocks, int block_size, int num_kv_heads, int slot_bytes, const int32_t* page_table, int max_pages,
+             const int32_t* seq_lens, int batch, const float* scores, int64_t score_batch_stride, int64_t score_head_stride, int max_tokens,
+             int keep, int recent, const int32_t* out_page_table, int out_max_pages, float* out_scores, int64_t out_batch_stride,
+             int64_t out_head_stride, int32_t* kept, int32_t* new_lens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Sequences and page ids that these operators left out since the library was loaded: {tq_cross, tq_decode_scored, tq_evict}; synchronises. */
+int tq_state_fault_counts(int32_t* counts3);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@ a tensor is not on a CUDA device the call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 
@@ -33,7 +34,7 @@ EXPORTS = (
     "tq_nc_write_kv_cache", "tq_nc_decode_workspace_bytes", "tq_nc_decode_paged", "tq_nc_write_dropped", "tq_exchange_bytes", "tq_decode_paged_exchange",
     "tq_dequant_paged", "tq_pages_packed_bytes", "tq_pages_gather", "tq_pages_scatter",
     "tq_decode_max_query_columns", "tq_set_exchange_wait_limit", "tq_decode_static_status", "tq_fault_counts",
-    "tq_write_guard_stats", "tq_pages_packed_bytes_for_slot",
+    "tq_write_guard_stats", "tq_pages_packed_bytes_for_slot", "tq_evict_workspace_bytes", "tq_evict", "tq_state_fault_counts",
 )
 
 _lib = None
@@ -543,6 +544,85 @@ def decode_static_status(device=None) -> int:
     word = torch.zeros(1, dtype=torch.int32, device=dev)
     _check(lib().tq_decode_static_status(_ptr(word), _stream(word)))
     return int(word.item())
+
+
+def state_fault_counts():
+    """(cross, scored decode, eviction): sequences and page ids that these operators left out, out of range, since the library was
+    loaded; synchronises."""
+    c = (ctypes.c_int32 * 3)()
+    _check(lib().tq_state_fault_counts(c))
+    return tuple(int(x) for x in c)
+
+
+def _same_device(t: torch.Tensor, others) -> None:
+    for o, name in others:
+        if o is not None:
+            _cuda(o, name)
+            if o.device != t.device:
+                raise TurboQuantError(f"{name} is on {o.device}, the cache on {t.device}")
+
+
+def _paged(kv_cache, page_table, seq_lens) -> None:
+    if kv_cache.dim() != 5 or kv_cache.shape[0] != 2 or not kv_cache.is_contiguous() or kv_cache.element_size() != 1:
+        raise TurboQuantError("kv_cache must be contiguous 1-byte [2, num_blocks, block_size, heads, slot_bytes]")
+    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+        raise TurboQuantError("seq_lens must be contiguous int32 [batch]")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.shape[0] != seq_lens.shape[0]:
+        raise TurboQuantError("the page table must be contiguous int32 [batch, pages]")
+
+
+def _scores(scores, name: str, batch: int, heads: int) -> None:
+    if scores.dtype != torch.float32 or scores.dim() != 3 or scores.shape[:2] != (batch, heads):
+        raise TurboQuantError(f"{name} must be fp32 [{batch}, {heads}, tokens], got {scores.dtype} {tuple(scores.shape)}")
+    if scores.shape[2] > 1 and scores.stride(2) != 1:
+        raise TurboQuantError(f"{name}: the scores of a row must be contiguous")
+
+
+def _on(device):
+    """Makes ``device`` the current one for the launches of a call."""
+    return torch.cuda.device(device) if torch.cuda.current_device() != device.index else contextlib.nullcontext()
+
+
+def evict(kv_cache, page_table, seq_lens, scores, keep: int, recent: int, out_page_table, out_scores, kept, new_lens) -> None:
+    """Of every sequence and KV head the last ``recent`` tokens and the best-scored others, ``keep`` in all, to positions 0, 1, ... of the pages of
+    ``out_page_table`` (None: the sequence's own), their scores to ``out_scores`` (may be ``scores``)."""
+    _cuda(kv_cache, "kv_cache")
+    _same_device(kv_cache, ((page_table, "page_table"), (seq_lens, "seq_lens"), (scores, "scores"), (out_page_table, "out_page_table"),
+                            (out_scores, "out_scores"), (kept, "kept"), (new_lens, "new_lens")))
+    _paged(kv_cache, page_table, seq_lens)
+    _, nb, bs, H, slot = kv_cache.shape
+    B = seq_lens.shape[0]
+    _scores(scores, "scores", B, H)
+    _scores(out_scores, "out_scores", B, H)
+    if not 1 <= keep < 1 << 31:
+        raise TurboQuantError(f"keep must be at least 1, got {keep}")
+    if not 0 <= recent <= keep:
+        raise TurboQuantError(f"recent must be in 0 ... keep = {keep}, got {recent}")
+    if out_page_table is not None:
+        _paged(kv_cache, out_page_table, seq_lens)
+        if B and out_page_table.data_ptr() == page_table.data_ptr():
+            raise TurboQuantError("the output table is the page table itself: leave it out to evict within the same pages")
+    if B == 0:
+        return
+    most = min(page_table.shape[1] * bs, scores.shape[2])
+    if out_scores.shape[2] < min(keep, most):
+        raise TurboQuantError(f"out_scores has room for {out_scores.shape[2]} tokens, {min(keep, most)} may stay")
+    for t, name, shape in ((kept, "kept", (B, H, keep)), (new_lens, "new_lens", (B,))):
+        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise TurboQuantError(f"{name} must be contiguous int32 {list(shape)}")
+    f = lib().tq_evict_workspace_bytes
+    f.restype = ctypes.c_size_t
+    shared = out_scores.untyped_storage().data_ptr() == scores.untyped_storage().data_ptr()
+    nbytes = f(ctypes.c_int(B), ctypes.c_int(H), ctypes.c_int(slot), ctypes.c_int(most), ctypes.c_int(keep), ctypes.c_int(out_page_table is None),
+               ctypes.c_int(shared))
+    with _on(kv_cache.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=kv_cache.device) if nbytes else None
+        _check(lib().tq_evict(
+            _ptr(kv_cache), ctypes.c_int64(nb), ctypes.c_int(bs), ctypes.c_int(H), ctypes.c_int(slot), _ptr(page_table), ctypes.c_int(page_table.shape[1]),
+            _ptr(seq_lens), ctypes.c_int(B), _ptr(scores), ctypes.c_int64(scores.stride(0)), ctypes.c_int64(scores.stride(1)),
+            ctypes.c_int(scores.shape[2]), ctypes.c_int(keep), ctypes.c_int(recent), _ptr(out_page_table),
+            ctypes.c_int(0 if out_page_table is None else out_page_table.shape[1]), _ptr(out_scores), ctypes.c_int64(out_scores.stride(0)),
+            ctypes.c_int64(out_scores.stride(1)), _ptr(kept), _ptr(new_lens), _ptr(ws), ctypes.c_size_t(nbytes), _stream(kv_cache)))
 
 
 # ---- the slot format of vLLM's native backend ("turboquant_4bit_nc"): one cache tensor ------------

@@ -38,6 +38,7 @@ UNITS = {
     "tq_decode_split.cu": [],
     "tq_dequant.cu": ["-fmad=false"],
     "tq_pages.cu": [],
+    "tq_evict.cu": [],
     "tq_generic.cu": ["-fmad=false"],
     "tq_nc.cu": ["-fmad=false"],
 }

@@ -214,6 +214,30 @@ class TurboQuantPagedAttention:
                             cu_seqlens.to(torch.int32), self.signs(dev), k, v, max_pages=block_table.shape[-1])
         return k, v
 
+    def evict(self, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, scores: torch.Tensor,
+              keep: int, recent: int = 0, out_block_table: torch.Tensor | None = None,
+              out_scores: torch.Tensor | None = None):
+        """The tokens of the lowest scores leave the cache.  For every sequence and KV head the last ``recent`` tokens stay and, of
+        the others, those of the largest ``scores`` (fp32 [batch, kv_heads, tokens], as ``decode_scored`` accumulates them), ``keep`` in
+        all or the whole sequence where it is shorter; a tie goes to the lower position, a NaN counts as -inf.  What stays keeps
+        its order and moves to positions 0, 1, ... of the pages of ``out_block_table`` (pages that the call does not read, so that
+        shared pages stay as they are), or of the sequence's own pages (None); the scores go with it to ``out_scores`` (None: in
+        place).  Returns ``(kept, lens)``: the positions that the tokens had, int32 [batch, kv_heads, keep], -1 behind the last one, and the new
+        lengths, int32 [batch].  Slots and scores behind them are left as they were."""
+        if block_table.dtype != torch.int32:
+            block_table = block_table.to(torch.int32)
+        if seq_lens.dtype != torch.int32:
+            seq_lens = seq_lens.to(torch.int32)
+        if out_block_table is not None:
+            out_block_table = out_block_table.to(torch.int32).contiguous()
+        if kv_cache.shape[3:4] != (self.num_kv_heads,):
+            raise _cabi.TurboQuantError(f"kv_cache must have {self.num_kv_heads} heads, got {tuple(kv_cache.shape)}")
+        kept = torch.empty((seq_lens.shape[0], self.num_kv_heads, max(int(keep), 0)), dtype=torch.int32, device=kv_cache.device)
+        lens = torch.empty(seq_lens.shape[0], dtype=torch.int32, device=kv_cache.device)
+        _cabi.evict(self._as_bytes(kv_cache), block_table.contiguous(), seq_lens.contiguous(), scores, int(keep), int(recent),
+                    out_block_table, scores if out_scores is None else out_scores, kept, lens)
+        return kept, lens
+
     def offload_pages(self, kv_cache: torch.Tensor, page_ids: torch.Tensor, host: torch.Tensor | None = None):
         """Packed copy of pages ``page_ids`` (K and V halves, 68 bytes per slot) in pinned host
         memory; asynchronous on the current stream (synchronise before reading ``host``).  The
