@@ -376,6 +376,25 @@ int tq_nc_decode_paged(const void* q, int q_dtype, int batch, int num_q_heads, i
 int tq_nc_write_dropped(int32_t* count);
 
 /* ---------------------------------------------------------------------------------------
+ * Paged decode attention that scores the cached tokens: tq_decode_paged, and
+ *   scores[b][h][t] += sum over the query heads of KV head h of softmax weight(t),   t < seq_lens[b]
+ * where the last new_tokens of a sequence begin at zero (the token just written has no score yet: 1).
+ *   page_table    int32 [batch][max_pages]
+ *   scores        fp32, element [b * batch stride + h * head stride + position], score_tokens positions a row
+ *   out_lse       optional fp32 [batch][num_q_heads], natural log
+ * head_dim 65 ... 128 (80-byte slots), any number of KV heads, up to 8 query heads on each.  Logits are worked out to about 2^-20, so that scores are fp32
+ * sums in earnest; out is as exact as its 16-bit types.  Results do not depend on an order of atomics.  Scores behind a sequence are left as they are.  A
+ * sequence longer than its page table, or of a negative length, has output zero and no weights; one longer than its scores has its output and
+ * leaves its scores alone; both are counted, and so is a page id outside [0, num_blocks), for which page 0 is read (tq_state_fault_counts).
+ * The workspace (tq_decode_scored_workspace_bytes; 256-byte aligned, no initialising) holds a logit for every query head and slot of the page table.
+ * No counterpart in the reference. */
+size_t tq_decode_scored_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_pages);
+int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q_heads, int num_kv_heads, int head_dim, const void* kv_cache,
+                     int64_t num_blocks, int block_size, int slot_bytes, const int32_t* page_table, int max_pages, const int32_t* seq_lens,
+                     const float* signs, float sm_scale, float* scores, int64_t score_batch_stride, int64_t score_head_stride, int score_tokens,
+                     int new_tokens, void* workspace, size_t workspace_bytes, void* out, int out_dtype, float* out_lse, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Eviction by accumulated attention weight.  Of every sequence's len tokens, for each KV head, the last
  * `recent` stay and of the others those of the largest scores, min(len, keep) in all; a tie goes to the lower
  * position, a NaN counts as -inf.  What stays keeps its order and moves to positions 0, 1, ... : whole slots of K and V, in the pages of

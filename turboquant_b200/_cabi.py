@@ -34,7 +34,8 @@ EXPORTS = (
     "tq_nc_write_kv_cache", "tq_nc_decode_workspace_bytes", "tq_nc_decode_paged", "tq_nc_write_dropped", "tq_exchange_bytes", "tq_decode_paged_exchange",
     "tq_dequant_paged", "tq_pages_packed_bytes", "tq_pages_gather", "tq_pages_scatter",
     "tq_decode_max_query_columns", "tq_set_exchange_wait_limit", "tq_decode_static_status", "tq_fault_counts",
-    "tq_write_guard_stats", "tq_pages_packed_bytes_for_slot", "tq_evict_workspace_bytes", "tq_evict", "tq_state_fault_counts",
+    "tq_write_guard_stats", "tq_pages_packed_bytes_for_slot", "tq_decode_scored_workspace_bytes", "tq_decode_scored", "tq_evict_workspace_bytes",
+    "tq_evict", "tq_state_fault_counts",
 )
 
 _lib = None
@@ -581,6 +582,50 @@ def _scores(scores, name: str, batch: int, heads: int) -> None:
 def _on(device):
     """Makes ``device`` the current one for the launches of a call."""
     return torch.cuda.device(device) if torch.cuda.current_device() != device.index else contextlib.nullcontext()
+
+
+def _query_rows(q, out, out_lse, signs) -> None:
+    if q.dim() != 3 or not q.is_contiguous():
+        raise TurboQuantError("q must be contiguous [rows, num_q_heads, head_dim]")
+    if out.shape != q.shape or not out.is_contiguous():
+        raise TurboQuantError(f"out must be contiguous {list(q.shape)}, got {list(out.shape)}")
+    if out_lse is not None and (out_lse.dtype != torch.float32 or out_lse.numel() != q.shape[0] * q.shape[1] or not out_lse.is_contiguous()):
+        raise TurboQuantError(f"out_lse must be contiguous fp32 [{q.shape[0]}, {q.shape[1]}]")
+    padded = 1 << (q.shape[2] - 1).bit_length()
+    if signs.dtype != torch.float32 or signs.numel() < padded or not signs.is_contiguous():
+        raise TurboQuantError(f"signs must be contiguous fp32 with {padded} entries (the padded head size)")
+
+
+def decode_scored(q, kv_cache, page_table, seq_lens, signs, sm_scale: float, scores, out, out_lse=None, new_tokens: int = 1):
+    """One decode step (``q`` / ``out`` [batch, Hq, D]) that adds every cached token's softmax weight, summed over the query heads of its KV
+    head, to ``scores`` (fp32 [batch, H, tokens]); the last ``new_tokens`` of a sequence begin at zero."""
+    _cuda(kv_cache, "kv_cache")
+    _same_device(kv_cache, ((q, "q"), (page_table, "page_table"), (seq_lens, "seq_lens"), (signs, "signs"), (scores, "scores"), (out, "out"),
+                            (out_lse, "out_lse")))
+    _paged(kv_cache, page_table, seq_lens)
+    _query_rows(q, out, out_lse, signs)
+    _, nb, bs, H, slot = kv_cache.shape
+    B, Hq, D = q.shape
+    if seq_lens.shape[0] != B:
+        raise TurboQuantError("seq_lens must have one entry per query row")
+    _scores(scores, "scores", B, H)
+    if new_tokens < 0:
+        raise TurboQuantError(f"new_tokens must not be negative, got {new_tokens}")
+    if debug_checks():
+        _check_pages(page_table, None, page_table.shape[1], seq_lens, nb, bs)
+    if B == 0:
+        return out
+    f = lib().tq_decode_scored_workspace_bytes
+    f.restype = ctypes.c_size_t
+    with _on(kv_cache.device):
+        nbytes = f(ctypes.c_int(B), ctypes.c_int(Hq), ctypes.c_int(H), ctypes.c_int(page_table.shape[1]))
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=kv_cache.device)
+        _check(lib().tq_decode_scored(
+            _ptr(q), ctypes.c_int(dtype_code(q.dtype)), ctypes.c_int(B), ctypes.c_int(Hq), ctypes.c_int(H), ctypes.c_int(D), _ptr(kv_cache),
+            ctypes.c_int64(nb), ctypes.c_int(bs), ctypes.c_int(slot), _ptr(page_table), ctypes.c_int(page_table.shape[1]), _ptr(seq_lens), _ptr(signs),
+            ctypes.c_float(sm_scale), _ptr(scores), ctypes.c_int64(scores.stride(0)), ctypes.c_int64(scores.stride(1)), ctypes.c_int(scores.shape[2]),
+            ctypes.c_int(new_tokens), _ptr(ws), ctypes.c_size_t(nbytes), _ptr(out), ctypes.c_int(dtype_code(out.dtype)), _ptr(out_lse), _stream(kv_cache)))
+    return out
 
 
 def evict(kv_cache, page_table, seq_lens, scores, keep: int, recent: int, out_page_table, out_scores, kept, new_lens) -> None:

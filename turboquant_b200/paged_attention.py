@@ -214,6 +214,29 @@ class TurboQuantPagedAttention:
                             cu_seqlens.to(torch.int32), self.signs(dev), k, v, max_pages=block_table.shape[-1])
         return k, v
 
+    def decode_scored(self, query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                      scores: torch.Tensor, output: torch.Tensor | None = None, out_lse: torch.Tensor | None = None,
+                      new_tokens: int = 1) -> torch.Tensor:
+        """``decode`` (one query a row, head sizes 65 ... 128) that also scores the cached tokens, for ``evict``: to ``scores`` (fp32
+        [batch, kv_heads, tokens], row b beside row b of the batch) is added every token's softmax weight, summed over the query
+        heads of its KV head.  The last ``new_tokens`` of a sequence begin at zero, whatever ``scores`` holds for them: the token just written is
+        one.  Scores behind a sequence are left as they were.  Its scratch, one fp32 logit for every query head and slot of the
+        block table among it, comes from torch's allocator at each call: calls on several streams and captured graphs do not share it."""
+        if query.dim() == 2:
+            query = query.view(query.shape[0], self.num_heads, self.head_size)
+        if query.shape[1:] != (self.num_heads, self.head_size) or kv_cache.shape[3:4] != (self.num_kv_heads,):
+            raise _cabi.TurboQuantError(f"query must be [batch, {self.num_heads}, {self.head_size}] and the cache have {self.num_kv_heads} heads, "
+                                        f"got {tuple(query.shape)} and {tuple(kv_cache.shape)}")
+        if output is None:
+            output = torch.empty_like(query, memory_format=torch.contiguous_format)
+        if block_table.dtype != torch.int32:
+            block_table = block_table.to(torch.int32)
+        if seq_lens.dtype != torch.int32:
+            seq_lens = seq_lens.to(torch.int32)
+        _cabi.decode_scored(query.contiguous(), self._as_bytes(kv_cache), block_table.contiguous(), seq_lens.contiguous(), self.signs(query.device),
+                            self.scale, scores, output.view(query.shape), out_lse, new_tokens)
+        return output
+
     def evict(self, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, scores: torch.Tensor,
               keep: int, recent: int = 0, out_block_table: torch.Tensor | None = None,
               out_scores: torch.Tensor | None = None):
