@@ -376,6 +376,24 @@ int tq_nc_decode_paged(const void* q, int q_dtype, int batch, int num_q_heads, i
 int tq_nc_write_dropped(int32_t* count);
 
 /* ---------------------------------------------------------------------------------------
+ * Cross attention: the query rows of a sequence (a decoder's prompt, any number) over all of its cached tokens (an encoder's states), no mask:
+ *   out[t, hq, :] = softmax(q[t, hq] . K^[b]^T * sm_scale) V^[b],     cu_seqlens_q[b] <= t < cu_seqlens_q[b + 1]
+ *   q, out        [total_q][num_q_heads][head_dim]; out_lse optional fp32 [total_q][num_q_heads], natural log
+ *   cu_seqlens_q  int32 [batch + 1], page_table int32 [batch][max_pages], seq_lens int32 [batch] (device)
+ *   total_tokens  at least the sum of seq_lens (host; sizes the workspace)
+ * head_dim 65 ... 128 (80-byte slots), any number of KV heads and of query heads on each.  Products are fp16 on the tensor cores with fp32 sums; with a bf16
+ * result queries, keys, values and probabilities are rounded to fp16 once each, with any other the probabilities alone.  A
+ * sequence without tokens gives zeros (LSE -inf); rows that belong to no sequence are left as they are.  A negative length, one
+ * beyond the page table or beyond total_tokens counts as no tokens, a range of cu_seqlens_q that is none as no rows, and a page id outside [0, num_blocks) reads
+ * page 0; all are counted (tq_state_fault_counts).  The workspace (tq_cross_workspace_bytes; 256-byte aligned, no initialising) holds the cached
+ * tokens as 16-bit rows.  The reference attends fresh keys and values only (turboquant/vllm_backend_fused.py:336-369). */
+size_t tq_cross_workspace_bytes(int batch, int total_q, int64_t total_tokens, int num_q_heads, int num_kv_heads, int max_pages, int out_dtype);
+int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* cu_seqlens_q, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+             const void* kv_cache, int64_t num_blocks, int block_size, int slot_bytes, const int32_t* page_table, int max_pages,
+             const int32_t* seq_lens, int64_t total_tokens, const float* signs, float sm_scale, void* workspace, size_t workspace_bytes, void* out,
+             int out_dtype, float* out_lse, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Paged decode attention that scores the cached tokens: tq_decode_paged, and
  *   scores[b][h][t] += sum over the query heads of KV head h of softmax weight(t),   t < seq_lens[b]
  * where the last new_tokens of a sequence begin at zero (the token just written has no score yet: 1).

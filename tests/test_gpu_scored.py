@@ -4,7 +4,8 @@ Bounds.  A logit: levels and queries are kept to 2^-21 (two fp16 parts each), th
 2^-22 of the sum of magnitudes S = scale sum |q k|: |dx| <= (2 * 2^-21 + 16 * 2^-22) S < 2^-17 S.  The rotation mixes the dims, so S is that of
 the vectors' lengths, scale |q| |k|.  A weight w = exp(x - lse): |dw| <= w (2 |dx| + 2^-20), the last for two exponentials and a logarithm; a weight
 below 2^-126, the least normal 32-bit value, becomes zero, which is 2^-126 at most for each of a score's heads.
-An output row: V's levels are within 2^-13 of their fp16 form, P within 2^-11, the weights as above, each relative to sum w |v|; and half a
+An output row: V's levels in fp16 are 4e-5 of a row's length off (codes of N(0, 1)
+rows), within 2^-13, P within 2^-11, the weights as above, each relative to sum w |v|; and half a
 step of its type."""
 import math
 

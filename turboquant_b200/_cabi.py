@@ -34,7 +34,8 @@ EXPORTS = (
     "tq_nc_write_kv_cache", "tq_nc_decode_workspace_bytes", "tq_nc_decode_paged", "tq_nc_write_dropped", "tq_exchange_bytes", "tq_decode_paged_exchange",
     "tq_dequant_paged", "tq_pages_packed_bytes", "tq_pages_gather", "tq_pages_scatter",
     "tq_decode_max_query_columns", "tq_set_exchange_wait_limit", "tq_decode_static_status", "tq_fault_counts",
-    "tq_write_guard_stats", "tq_pages_packed_bytes_for_slot", "tq_decode_scored_workspace_bytes", "tq_decode_scored", "tq_evict_workspace_bytes",
+    "tq_write_guard_stats", "tq_pages_packed_bytes_for_slot", "tq_cross_workspace_bytes", "tq_cross",
+    "tq_decode_scored_workspace_bytes", "tq_decode_scored", "tq_evict_workspace_bytes",
     "tq_evict", "tq_state_fault_counts",
 )
 
@@ -594,6 +595,39 @@ def _query_rows(q, out, out_lse, signs) -> None:
     padded = 1 << (q.shape[2] - 1).bit_length()
     if signs.dtype != torch.float32 or signs.numel() < padded or not signs.is_contiguous():
         raise TurboQuantError(f"signs must be contiguous fp32 with {padded} entries (the padded head size)")
+
+
+def cross(q, cu_seqlens_q, kv_cache, page_table, seq_lens, total_tokens: int, signs, sm_scale: float, out, out_lse=None):
+    """``q`` / ``out`` [rows, Hq, D]: rows cu_seqlens_q[b] ... of sequence b over all of its cached tokens; ``total_tokens`` is at least the
+    sum of ``seq_lens``."""
+    _cuda(kv_cache, "kv_cache")
+    _same_device(kv_cache, ((q, "q"), (cu_seqlens_q, "cu_seqlens_q"), (page_table, "page_table"), (seq_lens, "seq_lens"), (signs, "signs"), (out, "out"),
+                            (out_lse, "out_lse")))
+    _paged(kv_cache, page_table, seq_lens)
+    _query_rows(q, out, out_lse, signs)
+    _, nb, bs, H, slot = kv_cache.shape
+    T, Hq, D = q.shape
+    B = seq_lens.shape[0]
+    if cu_seqlens_q.dtype != torch.int32 or tuple(cu_seqlens_q.shape) != (B + 1,) or not cu_seqlens_q.is_contiguous():
+        raise TurboQuantError(f"cu_seqlens_q must be contiguous int32 [{B + 1}]")
+    if total_tokens < 0:
+        raise TurboQuantError(f"total_tokens must not be negative, got {total_tokens}")
+    if debug_checks():
+        _check_pages(page_table, None, page_table.shape[1], seq_lens, nb, bs)
+    if B == 0 or T == 0:
+        return out
+    f = lib().tq_cross_workspace_bytes
+    f.restype = ctypes.c_size_t
+    with _on(kv_cache.device):
+        nbytes = f(ctypes.c_int(B), ctypes.c_int(T), ctypes.c_int64(total_tokens), ctypes.c_int(Hq), ctypes.c_int(H), ctypes.c_int(page_table.shape[1]),
+                   ctypes.c_int(dtype_code(out.dtype)))
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=kv_cache.device)
+        _check(lib().tq_cross(
+            _ptr(q), ctypes.c_int(dtype_code(q.dtype)), ctypes.c_int(T), _ptr(cu_seqlens_q), ctypes.c_int(B), ctypes.c_int(Hq), ctypes.c_int(H),
+            ctypes.c_int(D), _ptr(kv_cache), ctypes.c_int64(nb), ctypes.c_int(bs), ctypes.c_int(slot), _ptr(page_table), ctypes.c_int(page_table.shape[1]),
+            _ptr(seq_lens), ctypes.c_int64(total_tokens), _ptr(signs), ctypes.c_float(sm_scale), _ptr(ws), ctypes.c_size_t(nbytes), _ptr(out),
+            ctypes.c_int(dtype_code(out.dtype)), _ptr(out_lse), _stream(kv_cache)))
+    return out
 
 
 def decode_scored(q, kv_cache, page_table, seq_lens, signs, sm_scale: float, scores, out, out_lse=None, new_tokens: int = 1):

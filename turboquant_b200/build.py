@@ -39,6 +39,7 @@ UNITS = {
     "tq_dequant.cu": ["-fmad=false"],
     "tq_pages.cu": [],
     "tq_scored.cu": [],
+    "tq_cross.cu": [],
     "tq_evict.cu": [],
     "tq_generic.cu": ["-fmad=false"],
     "tq_nc.cu": ["-fmad=false"],
@@ -84,7 +85,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     LIB_DIR.mkdir(exist_ok=True)
     obj_dir = PKG / "build"
     obj_dir.mkdir(exist_ok=True)
-    deps = [CSRC / "tq_common.cuh", CSRC / "tq_rows.cuh", CSRC / "tq_decode_common.cuh", CSRC / "tq_split.cuh", HEADER, Path(__file__)]
+    deps = [CSRC / "tq_common.cuh", CSRC / "tq_rows.cuh", CSRC / "tq_decode_common.cuh", CSRC / "tq_split.cuh", CSRC / "tq_tcgen05.cuh", HEADER, Path(__file__)]
 
     def compile_one(item):
         name, extra = item

@@ -93,6 +93,7 @@ bool encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, con
 int write_fault_count(int32_t* out);
 int dequant_fault_count(int32_t* out);
 int pages_fault_count(int32_t* out);
+int cross_fault_count(int32_t* out);
 int scored_fault_count(int32_t* out);
 int evict_fault_count(int32_t* out);
 
@@ -108,8 +109,8 @@ extern "C" int tq_fault_counts(int32_t* counts3) {
 
 extern "C" int tq_state_fault_counts(int32_t* counts3) {
     TQ_REQUIRE(counts3 != nullptr, TQ_ERR_INVALID, "null pointer");
-    counts3[0] = 0;
-    const int rc = tq::scored_fault_count(counts3 + 1);
+    int rc = tq::cross_fault_count(counts3);
+    if (rc == TQ_OK) rc = tq::scored_fault_count(counts3 + 1);
     return rc == TQ_OK ? tq::evict_fault_count(counts3 + 2) : rc;
 }
 

@@ -214,6 +214,32 @@ class TurboQuantPagedAttention:
                             cu_seqlens.to(torch.int32), self.signs(dev), k, v, max_pages=block_table.shape[-1])
         return k, v
 
+    def cross(self, query: torch.Tensor, cu_seqlens_q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
+              seq_lens: torch.Tensor, total_tokens: int, output: torch.Tensor | None = None,
+              out_lse: torch.Tensor | None = None) -> torch.Tensor:
+        """Cross attention: any number of query rows a sequence over ALL of its cached tokens, whose number is another (a decoder's prompt over
+        an encoder's states).  ``query`` [rows, heads, head_size], head sizes 65 ... 128; row ``cu_seqlens_q[b] + i`` is query i of
+        sequence b.  ``total_tokens``, at least the sum of ``seq_lens``, is passed by the caller (no sync).  A sequence without tokens gives
+        zeros; rows behind ``cu_seqlens_q[-1]`` are left as they were.  Its scratch, the cached tokens as 16-bit rows among it (512
+        bytes a token and KV head), comes from torch's allocator at each call.  Single new tokens go to ``decode``, up to 32 query
+        columns that share a sequence to ``decode_shared``: they read the codes as they are."""
+        if query.dim() == 2:
+            query = query.view(query.shape[0], self.num_heads, self.head_size)
+        if query.shape[1:] != (self.num_heads, self.head_size) or kv_cache.shape[3:4] != (self.num_kv_heads,):
+            raise _cabi.TurboQuantError(f"query must be [rows, {self.num_heads}, {self.head_size}] and the cache have {self.num_kv_heads} heads, "
+                                        f"got {tuple(query.shape)} and {tuple(kv_cache.shape)}")
+        if output is None:
+            output = torch.empty_like(query, memory_format=torch.contiguous_format)
+        if block_table.dtype != torch.int32:
+            block_table = block_table.to(torch.int32)
+        if seq_lens.dtype != torch.int32:
+            seq_lens = seq_lens.to(torch.int32)
+        if cu_seqlens_q.dtype != torch.int32:
+            cu_seqlens_q = cu_seqlens_q.to(torch.int32)
+        _cabi.cross(query.contiguous(), cu_seqlens_q.contiguous(), self._as_bytes(kv_cache), block_table.contiguous(), seq_lens.contiguous(),
+                    int(total_tokens), self.signs(query.device), self.scale, output.view(query.shape), out_lse)
+        return output
+
     def decode_scored(self, query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                       scores: torch.Tensor, output: torch.Tensor | None = None, out_lse: torch.Tensor | None = None,
                       new_tokens: int = 1) -> torch.Tensor:
