@@ -11,11 +11,13 @@
 // back to the Python layer, which converts, allocates or raises with its message, and calls the same entry point.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <unordered_map>
 
@@ -27,6 +29,12 @@ decltype(&tq_write_kv_cache) fn_write = nullptr;
 decltype(&tq_decode_paged_multi) fn_multi = nullptr;
 decltype(&tq_decode_paged_causal) fn_causal = nullptr;
 decltype(&tq_dequant_paged) fn_dequant = nullptr;
+decltype(&tq_cross) fn_cross = nullptr;
+decltype(&tq_cross_workspace_bytes) fn_cross_bytes = nullptr;
+decltype(&tq_decode_scored) fn_scored = nullptr;
+decltype(&tq_decode_scored_workspace_bytes) fn_scored_bytes = nullptr;
+decltype(&tq_evict) fn_evict = nullptr;
+decltype(&tq_evict_workspace_bytes) fn_evict_bytes = nullptr;
 decltype(&tq_quantize_flat) fn_quantize = nullptr;
 decltype(&tq_dequantize_flat) fn_dequantize = nullptr;
 decltype(&tq_last_error) fn_last_error = nullptr;
@@ -249,6 +257,164 @@ PyObject* layer_dequant(PyObject* o, PyObject* const* args, Py_ssize_t n) {
 }
 
 // -------------------------------------------------------------------------------------------------
+// cross attention, scored decode, eviction: their scratch is allocated here, call by call
+// -------------------------------------------------------------------------------------------------
+bool current(int device) { return c10::cuda::current_device() == (c10::DeviceIndex)device; }      // another one is made current by the Python layer
+bool page_table(const at::Tensor* t, int device, int64_t batch) { return int32_table(t, device) && t->dim() == 2 && t->size(0) == batch && t->size(1) > 0; }
+bool score_rows(const at::Tensor* t, int device, int64_t batch, int64_t heads) {
+    return t && t->get_device() == device && t->scalar_type() == at::kFloat && t->dim() == 3 && t->size(0) == batch && t->size(1) == heads &&
+           (t->size(2) <= 1 || t->stride(2) == 1) && t->size(2) < (int64_t)1 << 31;
+}
+// q [rows, heads, size] of this geometry, its output (made here if None) and lse
+struct Rows {
+    const at::Tensor *q, *out;
+    at::Tensor fresh;
+    float* lse = nullptr;
+    bool take(const Layer* self, PyObject* query, PyObject* output, PyObject* out_lse, int device) {
+        q = cuda_tensor(query);
+        if (!q || q->dim() != 3 || q->get_device() != device || float_code(q->scalar_type()) < 0 || !q->is_contiguous() || q->size(1) != self->heads ||
+            q->size(2) != self->head_size || q->size(0) == 0 || q->size(0) >= (int64_t)1 << 31)
+            return false;
+        if (out_lse != Py_None) {
+            const at::Tensor* t = cuda_tensor(out_lse);
+            if (!t || t->get_device() != device || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->numel() != q->size(0) * self->heads) return false;
+            lse = static_cast<float*>(t->data_ptr());
+        }
+        if (output == Py_None) {
+            fresh = at::empty_like(*q);
+            out = &fresh;
+            return true;
+        }
+        out = cuda_tensor(output);
+        return out && out->get_device() == device && float_code(out->scalar_type()) >= 0 && out->is_contiguous() && out->sizes() == q->sizes();
+    }
+    PyObject* give(PyObject* output) { return fresh.defined() ? THPVariable_Wrap(std::move(fresh)) : Py_NewRef(output); }
+};
+at::Tensor scratch(size_t bytes, const at::Tensor& like) {
+    return at::empty({(int64_t)(bytes ? bytes : 1)}, at::TensorOptions().dtype(at::kByte).device(like.device()));
+}
+bool small_int(PyObject* o, int64_t most, int64_t& v) {
+    if (!PyLong_Check(o)) return false;
+    v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    return v >= 0 && v <= most;
+}
+
+// cross(query, cu_seqlens_q, kv_cache, block_table, seq_lens, total_tokens, output | None, out_lse | None) -> output, or None: not the plain case
+PyObject* layer_cross(PyObject* o, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Layer* self = reinterpret_cast<Layer*>(o);
+    if (n != 8 || debug_checks()) Py_RETURN_NONE;
+    const at::Tensor *cu = cuda_tensor(args[1]), *cache = cuda_tensor(args[2]), *table = cuda_tensor(args[3]), *lens = cuda_tensor(args[4]);
+    int64_t total;
+    if (!byte_cache(cache) || !small_int(args[5], (int64_t)1 << 40, total)) Py_RETURN_NONE;
+    const int dev = cache->get_device();
+    const at::Tensor& signs = self->signs[dev];
+    if (!current(dev) || !signs.defined() || cache->size(3) != self->kv_heads || !int32_table(lens, dev) || lens->dim() != 1) Py_RETURN_NONE;
+    const int64_t B = lens->size(0);
+    if (B == 0 || !page_table(table, dev, B) || !int32_table(cu, dev) || cu->dim() != 1 || cu->size(0) != B + 1) Py_RETURN_NONE;
+    Rows rows;
+    if (!rows.take(self, args[0], args[6], args[7], dev)) Py_RETURN_NONE;
+    const int T = (int)rows.q->size(0), out_dtype = float_code(rows.out->scalar_type());
+    const size_t bytes = fn_cross_bytes((int)B, T, total, self->heads, self->kv_heads, (int)table->size(1), out_dtype);
+    const at::Tensor ws = scratch(bytes, *cache);
+    void* stream = stream_of(dev);
+    int rc;
+    {
+        Gil gil;
+        rc = fn_cross(rows.q->data_ptr(), float_code(rows.q->scalar_type()), T, static_cast<const int32_t*>(cu->data_ptr()), (int)B, self->heads,
+                      self->kv_heads, self->head_size, cache->data_ptr(), cache->size(1), (int)cache->size(2), (int)cache->size(4),
+                      static_cast<const int32_t*>(table->data_ptr()), (int)table->size(1), static_cast<const int32_t*>(lens->data_ptr()), total,
+                      static_cast<const float*>(signs.data_ptr()), self->scale, ws.data_ptr(), bytes, rows.out->data_ptr(), out_dtype, rows.lse, stream);
+    }
+    return rc ? failed(rc) : rows.give(args[6]);
+    END_HANDLE_TH_ERRORS
+}
+
+// decode_scored(query, kv_cache, block_table, seq_lens, scores, output | None, out_lse | None, new_tokens) -> output, or None: not the plain case
+PyObject* layer_scored(PyObject* o, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Layer* self = reinterpret_cast<Layer*>(o);
+    if (n != 8 || debug_checks()) Py_RETURN_NONE;
+    const at::Tensor *cache = cuda_tensor(args[1]), *table = cuda_tensor(args[2]), *lens = cuda_tensor(args[3]), *scores = cuda_tensor(args[4]);
+    int64_t fresh_tokens;
+    if (!byte_cache(cache) || !small_int(args[7], INT32_MAX, fresh_tokens)) Py_RETURN_NONE;
+    const int dev = cache->get_device();
+    const at::Tensor& signs = self->signs[dev];
+    if (!current(dev) || !signs.defined() || cache->size(3) != self->kv_heads || !int32_table(lens, dev) || lens->dim() != 1) Py_RETURN_NONE;
+    const int64_t B = lens->size(0);
+    if (!page_table(table, dev, B) || !score_rows(scores, dev, B, self->kv_heads)) Py_RETURN_NONE;
+    Rows rows;
+    if (!rows.take(self, args[0], args[5], args[6], dev) || rows.q->size(0) != B) Py_RETURN_NONE;
+    const size_t bytes = fn_scored_bytes((int)B, self->heads, self->kv_heads, (int)table->size(1));
+    const at::Tensor ws = scratch(bytes, *cache);
+    void* stream = stream_of(dev);
+    int rc;
+    {
+        Gil gil;
+        rc = fn_scored(rows.q->data_ptr(), float_code(rows.q->scalar_type()), (int)B, self->heads, self->kv_heads, self->head_size, cache->data_ptr(),
+                       cache->size(1), (int)cache->size(2), (int)cache->size(4), static_cast<const int32_t*>(table->data_ptr()), (int)table->size(1),
+                       static_cast<const int32_t*>(lens->data_ptr()), static_cast<const float*>(signs.data_ptr()), self->scale,
+                       static_cast<float*>(scores->data_ptr()), scores->stride(0), scores->stride(1), (int)scores->size(2), (int)fresh_tokens, ws.data_ptr(),
+                       bytes, rows.out->data_ptr(), float_code(rows.out->scalar_type()), rows.lse, stream);
+    }
+    return rc ? failed(rc) : rows.give(args[5]);
+    END_HANDLE_TH_ERRORS
+}
+
+// evict(kv_cache, block_table, seq_lens, scores, keep, recent, out_block_table | None, out_scores | None) -> (kept, lens), or None: not the plain case
+PyObject* layer_evict(PyObject* o, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Layer* self = reinterpret_cast<Layer*>(o);
+    if (n != 8) Py_RETURN_NONE;
+    const at::Tensor *cache = cuda_tensor(args[0]), *table = cuda_tensor(args[1]), *lens = cuda_tensor(args[2]), *scores = cuda_tensor(args[3]);
+    int64_t keep, recent;
+    if (!byte_cache(cache) || !small_int(args[4], INT32_MAX, keep) || keep == 0 || !small_int(args[5], keep, recent)) Py_RETURN_NONE;
+    const int dev = cache->get_device();
+    const int64_t H = self->kv_heads;
+    if (!current(dev) || cache->size(3) != H || !int32_table(lens, dev) || lens->dim() != 1) Py_RETURN_NONE;
+    const int64_t B = lens->size(0);
+    if (B == 0 || !page_table(table, dev, B) || !score_rows(scores, dev, B, H)) Py_RETURN_NONE;
+    const at::Tensor *to_table = nullptr, *to_scores = scores;
+    if (args[6] != Py_None) {
+        to_table = cuda_tensor(args[6]);
+        if (!page_table(to_table, dev, B) || to_table->data_ptr() == table->data_ptr()) Py_RETURN_NONE;
+    }
+    const int64_t most = std::min(table->size(1) * cache->size(2), scores->size(2));
+    if (args[7] != Py_None) {
+        to_scores = cuda_tensor(args[7]);
+        if (!score_rows(to_scores, dev, B, H) || to_scores->size(2) < std::min(keep, most)) Py_RETURN_NONE;
+    }
+    const auto ints = at::TensorOptions().dtype(at::kInt).device(cache->device());
+    at::Tensor kept = at::empty({B, H, keep}, ints), left = at::empty({B}, ints);
+    const size_t bytes = fn_evict_bytes((int)B, (int)H, (int)cache->size(4), (int)std::min(most, (int64_t)INT32_MAX), (int)keep, to_table == nullptr,
+                                        to_scores->storage().data() == scores->storage().data());
+    at::Tensor ws;
+    if (bytes) ws = scratch(bytes, *cache);
+    void* stream = stream_of(dev);
+    int rc;
+    {
+        Gil gil;
+        rc = fn_evict(cache->data_ptr(), cache->size(1), (int)cache->size(2), (int)H, (int)cache->size(4), static_cast<const int32_t*>(table->data_ptr()),
+                      (int)table->size(1), static_cast<const int32_t*>(lens->data_ptr()), (int)B, static_cast<const float*>(scores->data_ptr()),
+                      scores->stride(0), scores->stride(1), (int)scores->size(2), (int)keep, (int)recent,
+                      to_table ? static_cast<const int32_t*>(to_table->data_ptr()) : nullptr, to_table ? (int)to_table->size(1) : 0,
+                      static_cast<float*>(to_scores->data_ptr()), to_scores->stride(0), to_scores->stride(1), static_cast<int32_t*>(kept.data_ptr()),
+                      static_cast<int32_t*>(left.data_ptr()), bytes ? ws.data_ptr() : nullptr, bytes, stream);
+    }
+    if (rc) return failed(rc);
+    PyObject *a = THPVariable_Wrap(std::move(kept)), *b = THPVariable_Wrap(std::move(left));
+    PyObject* pair = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// -------------------------------------------------------------------------------------------------
 // flat quantizer
 // -------------------------------------------------------------------------------------------------
 int64_t padded_dim(int64_t d) {
@@ -338,6 +504,8 @@ PyObject* bind(PyObject*, PyObject* args) {
     };
     if (!take("tq_write_kv_cache", fn_write) || !take("tq_decode_paged_multi", fn_multi) || !take("tq_decode_paged_causal", fn_causal) ||
         !take("tq_dequant_paged", fn_dequant) || !take("tq_quantize_flat", fn_quantize) || !take("tq_dequantize_flat", fn_dequantize) ||
+        !take("tq_cross", fn_cross) || !take("tq_cross_workspace_bytes", fn_cross_bytes) || !take("tq_decode_scored", fn_scored) ||
+        !take("tq_decode_scored_workspace_bytes", fn_scored_bytes) || !take("tq_evict", fn_evict) || !take("tq_evict_workspace_bytes", fn_evict_bytes) ||
         !take("tq_last_error", fn_last_error)) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "bind: an entry point is missing");
         return nullptr;
@@ -352,6 +520,9 @@ PyMethodDef layer_methods[] = {
     {"write", (PyCFunction)(void (*)())layer_write, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction)(void (*)())layer_decode, METH_FASTCALL, nullptr},
     {"dequant", (PyCFunction)(void (*)())layer_dequant, METH_FASTCALL, nullptr},
+    {"cross", (PyCFunction)(void (*)())layer_cross, METH_FASTCALL, nullptr},
+    {"decode_scored", (PyCFunction)(void (*)())layer_scored, METH_FASTCALL, nullptr},
+    {"evict", (PyCFunction)(void (*)())layer_evict, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyType_Slot layer_slots[] = {{Py_tp_new, (void*)layer_new}, {Py_tp_dealloc, (void*)layer_dealloc}, {Py_tp_methods, layer_methods}, {0, nullptr}};

@@ -223,6 +223,9 @@ class TurboQuantPagedAttention:
         zeros; rows behind ``cu_seqlens_q[-1]`` are left as they were.  Its scratch, the cached tokens as 16-bit rows among it (512
         bytes a token and KV head), comes from torch's allocator at each call.  Single new tokens go to ``decode``, up to 32 query
         columns that share a sequence to ``decode_shared``: they read the codes as they are."""
+        done = self._calls.cross(query, cu_seqlens_q, kv_cache, block_table, seq_lens, total_tokens, output, out_lse)
+        if done is not None:
+            return done
         if query.dim() == 2:
             query = query.view(query.shape[0], self.num_heads, self.head_size)
         if query.shape[1:] != (self.num_heads, self.head_size) or kv_cache.shape[3:4] != (self.num_kv_heads,):
@@ -248,6 +251,9 @@ class TurboQuantPagedAttention:
         heads of its KV head.  The last ``new_tokens`` of a sequence begin at zero, whatever ``scores`` holds for them: the token just written is
         one.  Scores behind a sequence are left as they were.  Its scratch, one fp32 logit for every query head and slot of the
         block table among it, comes from torch's allocator at each call: calls on several streams and captured graphs do not share it."""
+        done = self._calls.decode_scored(query, kv_cache, block_table, seq_lens, scores, output, out_lse, new_tokens)
+        if done is not None:
+            return done
         if query.dim() == 2:
             query = query.view(query.shape[0], self.num_heads, self.head_size)
         if query.shape[1:] != (self.num_heads, self.head_size) or kv_cache.shape[3:4] != (self.num_kv_heads,):
@@ -273,6 +279,9 @@ class TurboQuantPagedAttention:
         shared pages stay as they are), or of the sequence's own pages (None); the scores go with it to ``out_scores`` (None: in
         place).  Returns ``(kept, lens)``: the positions that the tokens had, int32 [batch, kv_heads, keep], -1 behind the last one, and the new
         lengths, int32 [batch].  Slots and scores behind them are left as they were."""
+        done = self._calls.evict(kv_cache, block_table, seq_lens, scores, keep, recent, out_block_table, out_scores)
+        if done is not None:
+            return done
         if block_table.dtype != torch.int32:
             block_table = block_table.to(torch.int32)
         if seq_lens.dtype != torch.int32:
