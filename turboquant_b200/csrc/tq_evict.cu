@@ -5,11 +5,12 @@
 // token kept[j] moves to position j, in other pages or in the sequence's own.  Attention over the cache does not care that another head
 // has another token at that position: a key carries its position with it.
 //
-//   select   A cluster of blocks for each (sequence, head) finds the score of rank k = keep - recent by its bits, eight at a time from the top:
-//            a histogram of the digit among the tokens that agree with the digits found so far, summed over the cluster through distributed shared
-//            memory, then the digit at which the count from above reaches k.  A score becomes an unsigned word that sorts as the float does.
-//            Then every warp counts what it keeps of its own run of tokens, the counts are summed over the warps and blocks in front, and
-//            the warp writes its tokens at consecutive places.  No order of atomics reaches the result.
+//   select   A cluster of blocks for each (sequence, head) finds the score of rank k = keep - recent by its bits from the top.  A score becomes an
+//            unsigned word that sorts as the float does.  The leading eleven bits (sign, exponent, two of the fraction) come from a histogram of all
+//            tokens, summed over the cluster through distributed shared memory; a second walk over the tokens counts those above that bin
+//            and lists those in it, a few in a hundred; the other bits, 8, 8 and 5 at a time, come from the lists.  Then the counts of what stays
+//            are summed over the warps and blocks in front, each of which has a run of tokens of its own, and in a third walk
+//            every warp writes its tokens at consecutive places.  No order of atomics reaches the result.
 //   move     A block for each page of the destination: all its slots of K and V, 16 bytes a thread and step, so that the stores cover
 //            whole lines; the loads are gathered slots.
 //
@@ -19,14 +20,16 @@
 
 namespace tq {
 
-constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
-constexpr int kEvictRun = 128;                 // tokens a warp takes at once: four a lane
-constexpr int kEvictDigits = 256;
+constexpr int kEvictThreads = 512;             // of a block of the selection, two an SM
+constexpr int kEvictRun = 128;                 // tokens of a warp's load: four a lane
+constexpr int kEvictAhead = 4;                 // loads in flight together
 constexpr int kEvictMaxCluster = 16;
-// The histogram has a column for every lane, so that 32 scores of one exponent (sums of softmax weights mostly share two or three) are 32 banks and
-// not one counter.
-constexpr int kEvictHistBytes = kEvictDigits * 32 * 4;
-constexpr int kEvictMostKeys = 48 * 1024;      // sort keys a block keeps in shared memory; a longer share is read again from L2 in every pass
+// First histogram: 2048 bins of eight columns (lane % 8), as sums of softmax weights share few exponents.  Then, in its place, that of eight bits with a
+// column for every lane, and the lists, one for each warp; a warp whose list does not hold its tokens walks over all of them instead.
+constexpr int kEvictBins = 2048, kEvictColumns = 8, kEvictDigits = 256;
+constexpr int kEvictHistBytes = kEvictBins * kEvictColumns * 4, kEvictDigitBytes = kEvictDigits * 32 * 4;
+constexpr int kEvictListBytes = kEvictHistBytes - kEvictDigitBytes;
+constexpr int kEvictMostKeys = 36 * 1024;      // sort keys a block keeps in shared memory beside them; longer shares are read from L2 in every walk
 
 struct EvictParams {
     uint8_t* kv_cache;
@@ -41,7 +44,7 @@ struct EvictParams {
     uint8_t* staging;              // rows on their way within the same pages: [page of the output][2][16][kv heads][slot]
     int64_t num_blocks, half_bytes, slab_bytes;
     int64_t score_b, score_h, to_b, to_h, out_b, out_h;
-    int batch, kv_heads, slot_bytes, max_pages, out_max_pages, out_pages, max_tokens, keep, recent, cluster, key_room, wide;
+    int batch, kv_heads, slot_bytes, max_pages, out_max_pages, out_pages, max_tokens, keep, recent, cluster, wide;
     int scores_staged;
 };
 
@@ -69,6 +72,29 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// The sum over the cluster's C blocks of N neighbouring counts each: all loads are on their way before the first is used.
+template <int N>
+__device__ __forceinline__ void cluster_sums(const int* local, int C, int (&sum)[N]) {
+    int part[kEvictMaxCluster][N];
+#pragma unroll
+    for (int r = 0; r < kEvictMaxCluster; r++) {
+#pragma unroll
+        for (int i = 0; i < N; i++) part[r][i] = 0;
+        if (r < C) {
+            uint32_t at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(r));
+            if constexpr (N == 4) asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(part[r][0]), "=r"(part[r][1]), "=r"(part[r][2]), "=r"(part[r][3]) : "r"(at) : "memory");
+            else if constexpr (N == 2) asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(part[r][0]), "=r"(part[r][1]) : "r"(at) : "memory");
+            else asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(part[r][0]) : "r"(at) : "memory");
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        sum[i] = 0;
+#pragma unroll
+        for (int r = 0; r < kEvictMaxCluster; r++) sum[i] += part[r][i];
+    }
+}
 __device__ __forceinline__ int cluster_load(const int* local, uint32_t rank) {
     uint32_t at;
     int v;
@@ -77,16 +103,19 @@ __device__ __forceinline__ int cluster_load(const int* local, uint32_t rank) {
     return v;
 }
 
-__global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
+template <bool KEPT>
+__global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const __grid_constant__ EvictParams p) {
+    constexpr int THREADS = kEvictThreads, kWarps = THREADS / 32, kList = kEvictListBytes / 4 / kWarps;
     extern __shared__ __align__(16) uint32_t evict_smem[];
-    uint32_t* const hist = evict_smem;                            // [digit][lane]
-    uint32_t* const keys = evict_smem + kEvictDigits * 32;        // the block's share
-    __shared__ int sums[2][kEvictDigits], counts[2], warp_gt[kEvictWarps], warp_eq[kEvictWarps], found[2];
+    uint32_t* const hist = evict_smem;                            // [bin][column], then [digit][lane]
+    uint32_t* const lists = evict_smem + kEvictDigitBytes / 4;
+    uint32_t* const keys = evict_smem + kEvictHistBytes / 4;      // the block's share, KEPT
+    __shared__ __align__(16) int sums[kEvictBins], sums8[2][kEvictDigits];
+    __shared__ int counts[2], warp_gt[32], warp_eq[32], found[2][2], above_s[2][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int C = p.cluster, rank = C > 1 ? (int)cluster_rank() : 0;
     const int unit = blockIdx.x / C, b = unit / p.kv_heads, h = unit - b * p.kv_heads;
-    grid_launch_dependents();
-    for (int i = tid; i < kEvictDigits * 32; i += kEvictThreads) hist[i] = 0;
+    for (int i = tid; i < kEvictHistBytes / 16; i += THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
     grid_dependency_wait();
 
     bool bad;
@@ -99,124 +128,241 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const __
     const float* const row = p.scores + b * p.score_b + h * p.score_h;
     float* const to = p.score_to + b * p.to_b + h * p.to_h;
     int32_t* const kept = p.kept + (int64_t)unit * p.keep;
-    const int me = rank * kEvictThreads + tid, all = C * kEvictThreads;
+    const int me = rank * THREADS + tid, all = C * THREADS;
+    // The blocks of the move are let in late: waiting ones would keep other selecting blocks out (or ask for another split of the SM's memory).
+    auto leave = [&] { grid_launch_dependents(); };
     for (int j = me; j < recent; j += all) {
         kept[k + j] = M + j;
         to[k + j] = row[M + j];
     }
     for (int j = n + me; j < p.keep; j += all) kept[j] = -1;
-    if (k == M) {                      // all of them (uniform over the cluster, as the ways out below are)
+    if (k == M) {                      // all of them (uniform over the cluster, as the way out below is)
         for (int j = me; j < k; j += all) {
             kept[j] = j;
             to[j] = row[j];
         }
+        leave();
         return;
     }
-    if (k == 0) return;
+    if (k == 0) {
+        leave();
+        return;
+    }
 
-    // This warp's run of tokens, and the block's.
-    const int W = ((M + kEvictWarps * C - 1) / (kEvictWarps * C) + kEvictRun - 1) / kEvictRun * kEvictRun;
-    const int64_t first = (int64_t)rank * kEvictWarps * W;
-    const int64_t begin64 = first + (int64_t)warp * W;
+    // This warp's run of tokens.
+    const int W = ((M + kWarps * C - 1) / (kWarps * C) + kEvictRun - 1) / kEvictRun * kEvictRun;
+    const int64_t begin64 = ((int64_t)rank * kWarps + warp) * W;
     const int begin = begin64 < M ? (int)begin64 : M, end = begin64 + W < M ? (int)(begin64 + W) : M;
-    const bool resident = kEvictWarps * W <= p.key_room;
     uint32_t* const my_keys = keys + (size_t)warp * W;
-    auto load = [&](int at, uint32_t (&key)[4]) {                // tokens at + 4 lane ...; past the run: nothing
-        const int i = at + 4 * lane;
-        if (p.wide && i + 3 < end) {
-            const float4 v = *reinterpret_cast<const float4*>(row + i);
-            key[0] = evict_key(v.x); key[1] = evict_key(v.y); key[2] = evict_key(v.z); key[3] = evict_key(v.w);
-        } else {
+    const bool wide = p.wide;
+    // Goes over the warp's tokens, four a lane in each of kEvictAhead runs: body(first token of the lane in a run, keys, a run).  Past the end the key is zero, which
+    // no score has.
+    auto walk = [&](bool from_keys, auto&& body) {
+        for (int at = begin; at < end; at += kEvictRun * kEvictAhead) {
+            uint32_t key[kEvictAhead][4];
+            if (KEPT && from_keys) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) key[e] = i + e < end ? evict_key(row[i + e]) : 0u;
-        }
-    };
-    auto again = [&](int at, uint32_t (&key)[4]) {
-        if (resident) {
-            const uint4 v = *reinterpret_cast<const uint4*>(my_keys + (at - begin) + 4 * lane);
-            key[0] = v.x; key[1] = v.y; key[2] = v.z; key[3] = v.w;
-        } else {
-            load(at, key);
-        }
-    };
-
-    uint32_t prefix = 0;
-    int left = k;                      // the rank looked for among the tokens that agree with the prefix
-    __syncthreads();                   // the histogram is zero
-    for (int pass = 0; pass < 4; pass++) {
-        const int shift = 24 - 8 * pass;
-        for (int at = begin; at < end; at += kEvictRun) {
-            uint32_t key[4];
-            if (pass == 0) {
-                load(at, key);
-                if (resident) *reinterpret_cast<uint4*>(my_keys + (at - begin) + 4 * lane) = make_uint4(key[0], key[1], key[2], key[3]);
+                for (int u = 0; u < kEvictAhead; u++) {
+                    const bool in = at + kEvictRun * u < end;
+                    const uint4 k4 = in ? *reinterpret_cast<const uint4*>(my_keys + (at - begin) + kEvictRun * u + 4 * lane) : make_uint4(0u, 0u, 0u, 0u);
+                    key[u][0] = k4.x; key[u][1] = k4.y; key[u][2] = k4.z; key[u][3] = k4.w;
+                }
+            } else if (wide && at + kEvictRun * kEvictAhead <= end) {
+                float4 v[kEvictAhead];
+#pragma unroll
+                for (int u = 0; u < kEvictAhead; u++) v[u] = *reinterpret_cast<const float4*>(row + at + kEvictRun * u + 4 * lane);
+#pragma unroll
+                for (int u = 0; u < kEvictAhead; u++) {
+                    key[u][0] = evict_key(v[u].x); key[u][1] = evict_key(v[u].y); key[u][2] = evict_key(v[u].z); key[u][3] = evict_key(v[u].w);
+                }
             } else {
-                again(at, key);
+#pragma unroll
+                for (int u = 0; u < kEvictAhead; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int i = at + kEvictRun * u + 4 * lane + e;
+                        key[u][e] = i < end ? evict_key(row[i]) : 0u;
+                    }
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (at + 4 * lane + e < end && (pass == 0 || key[e] >> (shift + 8) == prefix)) atomicAdd(&hist[((key[e] >> shift) & 255u) * 32 + lane], 1u);
+            for (int u = 0; u < kEvictAhead; u++) body(at + kEvictRun * u + 4 * lane, key[u]);
+        }
+    };
+    auto all_sync = [&] {
+        if (C > 1) cluster_sync();
+        else __syncthreads();
+    };
+    // Of counts by thread, the first thread's bins uppermost: how many lie above this thread's.  Two calls use different `turn`s.
+    auto above_all = [&](int mine, int turn) {
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        if (lane == 31) above_s[turn][warp] = upto;
+        __syncthreads();
+        const int t = lane < warp ? above_s[turn][lane] : 0;
+        return upto - mine + __reduce_add_sync(0xffffffffu, t);
+    };
+
+    // ---- the leading eleven bits ------------------------------------------------------------------------
+    __syncthreads();                   // the histogram is zero
+    walk(false, [&](int at, const uint32_t (&key)[4]) {
+        if (KEPT && at - 4 * lane < end) *reinterpret_cast<uint4*>(my_keys + (at - begin)) = make_uint4(key[0], key[1], key[2], key[3]);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (key[e] != 0u) atomicAdd(&hist[(key[e] >> 21) * kEvictColumns + (lane & (kEvictColumns - 1))], 1u);
+    });
+    __syncthreads();
+    constexpr int kMine = kEvictBins / THREADS;
+    int left = k;                      // the rank looked for among the tokens that agree with what is known of the key
+    {
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            const uint4* const at = reinterpret_cast<const uint4*>(hist + (tid + THREADS * i) * kEvictColumns);
+            const uint4 x = at[0], y = at[1];
+            sums[tid + THREADS * i] = (int)(x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w);
+        }
+        all_sync();
+        int up[kMine], c[kMine], mine = 0;      // bins 2047 - kMine tid - i, the uppermost first
+        const int* const at = &sums[kEvictBins - kMine * (tid + 1)];
+        if (C > 1) {
+            cluster_sums<kMine>(at, C, up);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kMine; i++) up[i] = at[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            c[i] = up[kMine - 1 - i];
+            mine += c[i];
+        }
+        // (the histogram becomes the digits', zero)
+        for (int i = tid; i < kEvictDigitBytes / 16; i += THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+        int above = above_all(mine, 0);
+        if (above < left && above + mine >= left) {
+#pragma unroll
+            for (int i = 0; i < kMine; i++) {
+                if (above < left && above + c[i] >= left) {
+                    found[0][0] = kEvictBins - 1 - kMine * tid - i;
+                    found[0][1] = left - above;
+                }
+                above += c[i];
+            }
         }
         __syncthreads();
-        {   // two threads a digit, 16 columns each
-            const int digit = tid >> 1;
+    }
+    uint32_t prefix = (uint32_t)found[0][0];
+    left = found[0][1];
+
+    // ---- what lies above, and the list of what lies in the bin ---------------------------------------------
+    const uint32_t lower = (1u << lane) - 1u;
+    uint32_t* const list = lists + warp * kList;
+    int gt = 0, listed = 0;
+    walk(true, [&](int, const uint32_t (&key)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) gt += key[e] >> 21 > prefix;
+        const bool in[4] = {key[0] >> 21 == prefix && key[0] != 0u, key[1] >> 21 == prefix && key[1] != 0u, key[2] >> 21 == prefix && key[2] != 0u,
+                            key[3] >> 21 == prefix && key[3] != 0u};
+        if (__any_sync(0xffffffffu, in[0] | in[1] | in[2] | in[3])) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t m = __ballot_sync(0xffffffffu, in[e]);
+                const int at = listed + __popc(m & lower);
+                if (in[e] && at < kList) list[at] = key[e];
+                listed += __popc(m);
+            }
+        }
+    });
+    const bool fits = listed <= kList;
+    __syncwarp();
+    auto candidates = [&](auto&& body) {       // body(key) of every token in the bin, and of some zeros
+        if (fits) {
+            for (int i = 0; i < listed; i += 32) body(i + lane < listed ? list[i + lane] : 0u);
+        } else {
+            const uint32_t bin = (uint32_t)found[0][0];
+            walk(true, [&](int, const uint32_t (&key)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) body(key[e] >> 21 == bin ? key[e] : 0u);
+            });
+        }
+    };
+
+    // ---- the other bits -----------------------------------------------------------------------------------
+    // A single block with no more tokens in the bin than threads compares each with all: one step in place of three.
+    bool done = false;
+    if (C == 1) {
+        if (lane == 0) warp_gt[warp] = listed;
+        __syncthreads();
+        const int others = lane < kWarps ? warp_gt[lane] : 0, total = __reduce_add_sync(0xffffffffu, others);
+        const int first = __reduce_add_sync(0xffffffffu, lane < warp ? others : 0);
+        done = total <= THREADS && !__any_sync(0xffffffffu, others > kList);
+        if (done) {                    // (the digits' histogram is not needed)
+            for (int i = lane; i < listed; i += 32) hist[first + i] = list[i];
+            if (tid < 4) hist[total + tid] = 0u;
+            __syncthreads();
+            const uint32_t key = tid < total ? hist[tid] : 0u;
+            int above = 0, same = 0;
+            for (int i = 0; i < total; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(hist + i);
+                above += (v.x > key) + (v.y > key) + (v.z > key) + (v.w > key);
+                same += (v.x == key) + (v.y == key) + (v.z == key) + (v.w == key);
+            }
+            if (tid < total && above < left && above + same >= left) {       // (all threads of that key write the same)
+                found[1][0] = (int)key;
+                found[1][1] = left - above;
+            }
+            __syncthreads();
+            prefix = (uint32_t)found[1][0];
+            left = found[1][1];
+        }
+    }
+    for (int pass = 0; pass < 3 && !done; pass++) {
+        const int shift = pass == 0 ? 13 : pass == 1 ? 5 : 0, bits = pass == 2 ? 5 : 8;
+        const uint32_t mask = (1u << bits) - 1u;
+        candidates([&](uint32_t key) {
+            if (key != 0u && key >> (shift + bits) == prefix) atomicAdd(&hist[((key >> shift) & mask) * 32 + lane], 1u);
+        });
+        __syncthreads();
+        {   // THREADS / 256 threads a digit, the columns shared out
+            constexpr int kShare = THREADS / kEvictDigits, kEach = 32 / kShare;
+            const int digit = tid / kShare, first_column = kEach * (tid % kShare);
             uint32_t sum = 0;
 #pragma unroll
-            for (int c = 0; c < 16; c++) {
-                const int at = digit * 32 + 16 * (tid & 1) + ((c + digit) & 15);
+            for (int c = 0; c < kEach; c++) {
+                const int at = digit * 32 + first_column + ((c + digit) & (kEach - 1));
                 sum += hist[at];
                 hist[at] = 0;
             }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            if ((tid & 1) == 0) sums[pass & 1][digit] = (int)sum;
+#pragma unroll
+            for (int o = 1; o < kShare; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (tid % kShare == 0) sums8[pass & 1][digit] = (int)sum;
         }
-        if (C > 1) cluster_sync();
-        else __syncthreads();
-        if (warp == 0) {               // lane l: digits 255 - 8 l downwards
-            int c[8], mine = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                c[e] = 0;
-                for (int r = 0; r < C; r++) c[e] += C > 1 ? cluster_load(&sums[pass & 1][255 - 8 * lane - e], (uint32_t)r) : sums[pass & 1][255 - 8 * lane - e];
-                mine += c[e];
-            }
-            int upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += t;
-            }
-            int above = upto - mine;
-            if (above < left && upto >= left) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if (above < left && above + c[e] >= left) {
-                        found[0] = 255 - 8 * lane - e;
-                        found[1] = left - above;
-                        break;
-                    }
-                    above += c[e];
-                }
-            }
+        all_sync();
+        int mine = 0;                  // thread t < 256: digit 255 - t
+        if (tid < kEvictDigits) {
+            int sum[1] = {sums8[pass & 1][255 - tid]};
+            if (C > 1) cluster_sums<1>(&sums8[pass & 1][255 - tid], C, sum);
+            mine = sum[0];
+        }
+        const int above = above_all(mine, ~pass & 1);
+        if (above < left && above + mine >= left) {
+            found[1][0] = 255 - tid;
+            found[1][1] = left - above;
         }
         __syncthreads();
-        prefix = prefix << 8 | (uint32_t)found[0];
-        left = found[1];
-        __syncthreads();               // found is read before the next pass writes it
+        prefix = prefix << bits | (uint32_t)found[1][0];
+        left = found[1][1];
+        __syncthreads();               // found is read before it is written again
     }
     // prefix is now the key of rank k, and `left` of the tokens that have it stay: those of the lowest positions.
 
-    int gt = 0, eq = 0;
-    for (int at = begin; at < end; at += kEvictRun) {
-        uint32_t key[4];
-        again(at, key);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const bool in = at + 4 * lane + e < end;
-            gt += in && key[e] > prefix;
-            eq += in && key[e] == prefix;
-        }
-    }
+    int eq = 0;
+    candidates([&](uint32_t key) {
+        gt += key > prefix;
+        eq += key == prefix;
+    });
     gt = __reduce_add_sync(0xffffffffu, gt);
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) {
@@ -225,7 +371,7 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const __
     }
     __syncthreads();
     if (warp == 0) {                   // sums of the warps in front, and the block's
-        int g = lane < kEvictWarps ? warp_gt[lane] : 0, q = lane < kEvictWarps ? warp_eq[lane] : 0;
+        int g = lane < kWarps ? warp_gt[lane] : 0, q = lane < kWarps ? warp_eq[lane] : 0;
         const int g0 = g, q0 = q;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -235,39 +381,32 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const __
                 q += c;
             }
         }
-        if (lane < kEvictWarps) {
-            warp_gt[lane] = g - g0;
-            warp_eq[lane] = q - q0;
-        }
+        warp_gt[lane] = g - g0;
+        warp_eq[lane] = q - q0;
         if (lane == 31) {
             counts[0] = g;
             counts[1] = q;
         }
     }
-    if (C > 1) cluster_sync();
-    else __syncthreads();
+    all_sync();
     int before_gt = warp_gt[warp], before_eq = warp_eq[warp];
-    for (int r = 0; r < rank; r++) {
-        before_gt += cluster_load(&counts[0], (uint32_t)r);
-        before_eq += cluster_load(&counts[1], (uint32_t)r);
+    if (C > 1) {
+        before_gt += __reduce_add_sync(0xffffffffu, lane < rank ? cluster_load(&counts[0], (uint32_t)min(lane, C - 1)) : 0);
+        before_eq += __reduce_add_sync(0xffffffffu, lane < rank ? cluster_load(&counts[1], (uint32_t)min(lane, C - 1)) : 0);
+        cluster_sync();                // no block of the cluster leaves while another reads its counts
     }
-    if (C > 1) cluster_sync();         // no block of the cluster leaves while another reads its counts
+    leave();
     int ties = left - before_eq;       // of this warp's tokens with the key of rank k, the first `ties` stay
     int place = before_gt + min(before_eq, left);
-    const uint32_t lower = (1u << lane) - 1u;
-    for (int at = begin; at < end; at += kEvictRun) {
-        uint32_t key[4];
-        again(at, key);
+    walk(true, [&](int at, const uint32_t (&key)[4]) {
         bool is_eq[4], stays[4];
-        int eq_before = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const bool in = at + 4 * lane + e < end;
-            stays[e] = in && key[e] > prefix;
-            is_eq[e] = in && key[e] == prefix;
+            stays[e] = key[e] > prefix;
+            is_eq[e] = key[e] == prefix;
         }
         if (__any_sync(0xffffffffu, is_eq[0] | is_eq[1] | is_eq[2] | is_eq[3])) {
-            int total = 0;
+            int total = 0, eq_before = 0;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t m = __ballot_sync(0xffffffffu, is_eq[e]);
@@ -288,15 +427,21 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const __
             j += __popc(m & lower);
             place += __popc(m);
         }
+        float score[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {   // the score from its key; a key that stands for two (zeros, a NaN and -inf) is looked up
+            score[e] = __uint_as_float(key[e] ^ (key[e] >> 31 ? 0x80000000u : 0xffffffffu));
+            if (stays[e] && (key[e] == 0x80000000u || key[e] == 0x007fffffu)) score[e] = row[at + e];
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             if (stays[e]) {
-                kept[j] = at + 4 * lane + e;
-                to[j] = row[at + 4 * lane + e];
+                kept[j] = at + e;
+                to[j] = score[e];
                 j++;
             }
         }
-    }
+    });
 }
 
 // One block for each page of the output.  STAGE 0: from the cache to the cache, 1: from the cache to the staging copy, 2: from there to the cache.
@@ -369,6 +514,56 @@ int evict_fault_count(int32_t* out) {
 }
 
 static size_t evict_up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Launches the selection with the largest cluster of up to C blocks of which all run at the same time.  too_long: a block's keys have no room in shared memory.
+template <bool KEPT>
+static int launch_select(EvictParams& p, int units, int C, int too_long, cudaStream_t s) {
+    // (A cluster stays inside one of the device's groups of SMs, which have not all the same number: eight of sixteen blocks would run seven and one.)
+    static int active[64][kEvictMaxCluster + 1] = {};      // by device: clusters of c blocks that run at the same time, plus one
+    int dev = 0;
+    TQ_CUDA(cudaGetDevice(&dev));
+    TQ_REQUIRE(dev >= 0 && dev < 64, TQ_ERR_UNSUPPORTED, "device %d", dev);
+    const auto kernel = evict_select_kernel<KEPT>;
+    constexpr int THREADS = kEvictThreads, kMost = kEvictHistBytes + (KEPT ? kEvictMostKeys * 4 : 0);
+    if (active[dev][1] == 0) {
+        TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+        TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        active[dev][1] = 1;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    auto share = [&](int c) { return ((p.max_tokens + THREADS / 32 * c - 1) / (THREADS / 32 * c) + kEvictRun - 1) / kEvictRun * kEvictRun * (THREADS / 32); };
+    for (; C > 1; C--) {
+        if (active[dev][C] == 0) {
+            cfg.gridDim = dim3((unsigned)(64 * C));
+            cfg.dynamicSmemBytes = KEPT ? kMost / 2 : kMost;      // (shares of up to a few thousand keys leave two an SM)
+            attr[0].val.clusterDim.x = (unsigned)C;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            active[dev][C] = n + 1;
+        }
+        if (active[dev][C] - 1 >= units) break;
+    }
+    if (KEPT && share(C) > kEvictMostKeys) return too_long;
+    p.cluster = C;
+    cfg.gridDim = dim3((unsigned)(units * C));
+    cfg.dynamicSmemBytes = KEPT ? kEvictHistBytes + (size_t)share(C) * 4 : (size_t)kMost;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    cfg.numAttrs = 2;
+    TQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    return TQ_OK;
+}
 
 template <int STAGE>
 static int launch_move(const EvictParams& p, cudaStream_t s) {
@@ -460,40 +655,18 @@ extern "C" int tq_evict(void* kv_cache, int64_t num_blocks, int block_size, int 
         p.to_b = out_batch_stride;
     }
 
-    // Blocks of a cluster: as many as leave each 4096 tokens, while all clusters together are at most two blocks an SM.
+    // Blocks of a cluster: as many as leave each 4096 tokens, up to an SM each.
     int sms = 0;
-    const int rc = device_sm_count(&sms);
+    int rc = device_sm_count(&sms);
     if (rc != TQ_OK) return rc;
     const int units = batch * num_kv_heads;
     int C = 1;
-    while (C < kEvictMaxCluster && most / (2 * C) >= 4096 && (int64_t)units * 2 * C <= 2 * sms) C *= 2;
-    p.cluster = C;
-    const int share = ((most + kEvictWarps * C - 1) / (kEvictWarps * C) + kEvictRun - 1) / kEvictRun * kEvictRun * kEvictWarps;
-    p.key_room = share <= kEvictMostKeys ? share : 0;
-    const size_t smem = kEvictHistBytes + (size_t)p.key_room * 4;
-    static bool configured[64] = {};
-    int dev = 0;
-    TQ_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
-        TQ_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictHistBytes + kEvictMostKeys * 4));
-        TQ_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        if (dev >= 0 && dev < 64) configured[dev] = true;
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(units * C));
-    cfg.blockDim = dim3(kEvictThreads);
-    cfg.dynamicSmemBytes = smem;
+    while (C < kEvictMaxCluster && most / (C + 1) >= 4096 && (int64_t)units * (C + 1) <= sms) C++;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)C;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    TQ_CUDA(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
+    constexpr int kTooLong = -1;
+    rc = launch_select<true>(p, units, C, kTooLong, s);
+    if (rc == kTooLong) rc = launch_select<false>(p, units, C, kTooLong, s);
+    if (rc != TQ_OK) return rc;
     if (!in_place) return launch_move<0>(p, s);
     const int moved = launch_move<1>(p, s);
     return moved != TQ_OK ? moved : launch_move<2>(p, s);
