@@ -34,6 +34,7 @@ static_assert(kScoredRing >= 8 * kHeadDim * 4, "a warp's partial output goes thr
 struct ScoredParams {
     SplitParams d;
     float* logits;             // [batch x KV heads][room][query heads of a KV head], base 2
+    int2* plan;                // [batch], up to kSplitSelf sequences: pages of the sequence, its place in the work list
     float* row_lse;            // [batch x KV heads][query heads of a KV head], base 2: rows that one group finished
     float* scores;
     int64_t score_b, score_h;
@@ -44,6 +45,11 @@ struct ScoredParams {
 
 static __device__ int32_t g_scored_faults = 0;
 
+// The slots of a page in one tensor copy, as in the split decode, but first to leave L2: read once, while the logits written meanwhile are read again.
+__device__ __forceinline__ void scored_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar), "l"(policy) : "memory");
+}
 // Four code bytes through both tables: the rest is 128 bytes behind the level.
 __device__ __forceinline__ void scored_lookup(uint32_t w, uint32_t lut_lane, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
 #pragma unroll
@@ -97,7 +103,7 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
     fence_barrier_init();
     __syncthreads();
     grid_dependency_wait();
-    grid_launch_dependents();    // the join reads seq_lens ahead of its own wait
+    grid_launch_dependents();
 
     SplitPlan s;
     if constexpr (MANY) split_plan_many<GW, NG>(p, s, lane);
@@ -116,6 +122,20 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
     if constexpr (MANY) {
         if (blockIdx.x == 0 && warp == 0) split_keep_plan(p, s);
         split_jump(p, s, pos < hi ? __ffs(__ballot_sync(0xffffffffu, s.ends > pos)) - 1 : 0);
+    } else if (blockIdx.x == gridDim.x - 1 && warp == 0) {      // for the join, whose blocks start when this kernel's end: there is no room beside them
+        if (lane == 0) {
+            p.header[1] = s.total;
+            p.header[2] = s.workers;
+            p.header[3] = s.piece;
+        }
+        SplitPlan all = s;
+        for (int first = 0;;) {
+            if (first + lane < p.batch) sp.plan[first + lane] = make_int2(all.np, all.vstart);
+            const int run = __shfl_sync(0xffffffffu, all.vend, 31);
+            first += 32;
+            if (first >= p.batch) break;
+            split_load(p, all, first, run, false);
+        }
     }
     int4* const plan = reinterpret_cast<int4*>(at_smem(kScoredPlan + (uint32_t)warp * 512u + (uint32_t)lane * 16u));
     *plan = make_int4(s.np, s.len, s.vstart, s.vend);
@@ -198,7 +218,7 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
             if (lane == 0 && i < n && !lost) {
                 const uint32_t bar = full_at + 8 * to;
                 split_expect(bar, kScoredStage);
-                split_box(ring_at + to * kScoredStage, &p.cache_map, x, id * kPageTokens, 0, bar);
+                scored_box(ring_at + to * kScoredStage, &p.cache_map, x, id * kPageTokens, bar, l2_policy_evict_first());
             }
         };
 #pragma unroll
@@ -457,10 +477,10 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
 
 // Joins the partials of the heads that were cut and adds the weights to the scores.  A block takes every chunks-th run of 256 tokens of one (sequence, KV
 // head): it works out the lse of the head's rows from the partials (they are few), writes the output rows r = chunk, chunk + chunks, ... , and
-// goes over its tokens' logits.  The plan is made ahead of the wait.
-constexpr int kJoinThreads = 256;
+// goes over its tokens' logits.
+constexpr int kJoinThreads = 256, kJoinAhead = 4;
 __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_constant__ ScoredParams sp) {
-    constexpr int PD = kHeadDim, E = PD / 32, GW = kScoredGroupWarps, NG = kScoredGroups, kWarps = kJoinThreads / 32;
+    constexpr int PD = kHeadDim, E = PD / 32, kWarps = kJoinThreads / 32;
     const SplitParams& p = sp.d;
     __shared__ float acc_s[kWarps][PD], sign_s[PD], lse_s[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -468,17 +488,25 @@ __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_
     grid_launch_dependents();
     const int bh = blockIdx.x / sp.chunks, chunk = blockIdx.x - bh * sp.chunks, b = bh / p.kv_heads, head = bh - b * p.kv_heads;
     for (int i = tid; i < PD; i += kJoinThreads) sign_s[i] = p.signs[i];
+    grid_dependency_wait();
+    const int given = p.seq_lens[b];
     SplitPlan s;
-    const bool many = p.batch > kSplitSelf;
-    if (many) {
-        grid_dependency_wait();
+    int np, vstart;
+    if (p.batch > kSplitSelf) {
         split_kept_plan(p, s, lane);
         split_jump(p, s, b / (32 * split_bin(p)));
+        while (s.base + 32 <= b) split_load(p, s, s.base + 32, __shfl_sync(0xffffffffu, s.vend, 31), false);
+        np = __shfl_sync(0xffffffffu, s.np, (b - s.base) & 31);
+        vstart = __shfl_sync(0xffffffffu, s.vstart, (b - s.base) & 31);
     } else {
-        split_plan<GW, NG>(p, s, lane);     // every decode block is past its wait: the lengths are final
+        const int2 place = sp.plan[b];
+        np = place.x;
+        vstart = place.y;
+        s.total = p.header[1];
+        s.workers = p.header[2];
+        s.piece = p.header[3];
+        s.head_set = s.piece ? 1 : p.head_set;
     }
-    while (s.base + 32 <= b) split_load(p, s, s.base + 32, __shfl_sync(0xffffffffu, s.vend, 31), false);
-    const int np = __shfl_sync(0xffffffffu, s.np, (b - s.base) & 31), vstart = __shfl_sync(0xffffffffu, s.vstart, (b - s.base) & 31);
     const int hs = s.head_set, hset = head / hs, hsub = head - hset * hs;
     int first = 0, count = 0;           // workers of this head's parts
     if (np > 0 && s.total > 0) {
@@ -491,10 +519,24 @@ __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_
             count = (int)((end * s.workers + s.total - 1) / s.total) - first;
         }
     }
-    if (!many) grid_dependency_wait();
-    const int given = p.seq_lens[b];
     const bool fits = given <= sp.score_room && np == (given > 0 ? (given + kPageTokens - 1) / kPageTokens : 0) && given >= 0;
     if (!fits && head == 0 && chunk == 0 && tid == 0) atomicAdd(&g_scored_faults, 1);
+    // The first tokens' logits and scores are on their way while the lse is worked out.
+    const int64_t step = (int64_t)sp.chunks * kJoinThreads, t_first = (int64_t)chunk * kJoinThreads + tid;
+    float* const score = sp.scores + b * sp.score_b + head * sp.score_h;
+    const float* const logits = sp.logits + (int64_t)bh * sp.room * G;
+    const int64_t old_end = (int64_t)given - sp.new_tokens;
+    float4 v[kJoinAhead];
+    float old[kJoinAhead];
+    auto fetch = [&](int64_t t0) {
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; u++) {
+            const int64_t t = t0 + step * u;
+            if (G == 4) v[u] = t < given ? *reinterpret_cast<const float4*>(logits + t * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            old[u] = t < old_end ? score[t] : 0.0f;
+        }
+    };
+    if (fits) fetch(t_first);
     auto slot_row = [&](int i, int r) -> int64_t { return ((int64_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * hs + hsub) * G + r; };
     for (int r = warp; r < G; r += kWarps) {
         float lse = -INFINITY;
@@ -540,22 +582,33 @@ __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_
         }
     }
     if (!fits) return;
-    float* const score = sp.scores + b * sp.score_b + head * sp.score_h;
-    const float* const logits = sp.logits + (int64_t)bh * sp.room * G;
     float lse[8];
 #pragma unroll
     for (int r = 0; r < 8; r++) lse[r] = r < G && lse_s[r] != -INFINITY ? lse_s[r] : INFINITY;      // a row without a weight: exp2(x - inf) = 0
-    for (int64_t t = (int64_t)chunk * kJoinThreads + tid; t < given; t += (int64_t)sp.chunks * kJoinThreads) {
-        float w = 0.0f;
+    for (int64_t t0 = t_first; t0 < given; t0 += step * kJoinAhead) {
+        float w[kJoinAhead];
+        if (t0 != t_first) fetch(t0);
         if (G == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(logits + t * 4);
-            w = (fast_exp2(v.x - lse[0]) + fast_exp2(v.y - lse[1])) + (fast_exp2(v.z - lse[2]) + fast_exp2(v.w - lse[3]));
-        } else {
 #pragma unroll
-            for (int r = 0; r < 8; r++)
-                if (r < G) w += fast_exp2(logits[t * G + r] - lse[r]);
+            for (int u = 0; u < kJoinAhead; u++)
+                w[u] = (fast_exp2(v[u].x - lse[0]) + fast_exp2(v[u].y - lse[1])) + (fast_exp2(v[u].z - lse[2]) + fast_exp2(v[u].w - lse[3]));
+        } else {
+            float x[kJoinAhead][8];
+#pragma unroll
+            for (int u = 0; u < kJoinAhead; u++)
+#pragma unroll
+                for (int r = 0; r < 8; r++) x[u][r] = r < G && t0 + step * u < given ? logits[(t0 + step * u) * G + r] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < kJoinAhead; u++) {
+                w[u] = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+                    if (r < G) w[u] += fast_exp2(x[u][r] - lse[r]);
+            }
         }
-        score[t] = t < given - sp.new_tokens ? score[t] + w : w;
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; u++)
+            if (t0 + step * u < given) score[t0 + step * u] = old[u] + w[u];
     }
 }
 
@@ -573,12 +626,13 @@ int scored_fault_count(int32_t* out) {
 }
 
 struct ScoredLayout {
-    size_t partial_lse, partial_o, row_lse, logits, end;
+    size_t plan, partial_lse, partial_o, row_lse, logits, end;
 };
 static ScoredLayout scored_layout(int batch, int heads, int kv_heads, int64_t max_pages, int ctas) {
     const size_t G = (size_t)(heads / kv_heads), rows = (size_t)2 * ctas * kScoredGroups * G;
     ScoredLayout l;
-    l.partial_lse = 256;
+    l.plan = 256;
+    l.partial_lse = l.plan + scored_up((size_t)kSplitSelf * sizeof(int2));
     l.partial_o = l.partial_lse + scored_up(rows * 4);
     l.row_lse = l.partial_o + scored_up(rows * kHeadDim * 4);
     l.logits = l.row_lse + scored_up((size_t)batch * heads * 4);
@@ -674,6 +728,7 @@ extern "C" int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q
     p.v_scale = (float)(inv / kLevelScale);
     p.k_scale = (float)(inv / kLevelScale * (double)sm_scale * 1.4426950408889634);
     sp.logits = reinterpret_cast<float*>(ws + lay.logits);
+    sp.plan = reinterpret_cast<int2*>(ws + lay.plan);
     sp.row_lse = reinterpret_cast<float*>(ws + lay.row_lse);
     sp.scores = scores;
     sp.score_b = score_batch_stride;
@@ -681,7 +736,7 @@ extern "C" int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q
     sp.room = (int64_t)max_pages * kPageTokens;
     sp.score_room = score_tokens;
     sp.new_tokens = new_tokens;
-    // A block of the join for every 256 tokens, up to eight blocks an SM in all (and one a row at least, where a row is more than that).
+    // A block of the join for every 256 tokens, up to eight an SM in all (and one a row at least).
     const int64_t runs = (most + kJoinThreads - 1) / kJoinThreads, fit = (int64_t)8 * sms / ((int64_t)batch * num_kv_heads);
     sp.chunks = (int)(runs < 1 ? 1 : runs < (fit > 1 ? fit : 1) ? runs : (fit > 1 ? fit : 1));
     rc = encode_cache_map(&p.cache_map, kv_cache, num_blocks, (int64_t)num_kv_heads * slot_bytes, kScoredRow, 2);
