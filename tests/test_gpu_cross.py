@@ -102,6 +102,42 @@ def test_tiles_and_lengths(q_lens, lens, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q_lens, lens, Hq, H, D", [([200], [1], 8, 2, 128), ([150], [128], 8, 2, 128), ([400], [300], 4, 2, 96), ([700, 1, 0, 300], [129, 700, 40, 0], 8, 2, 128),
+                                                    ([2500, 40], [400, 200], 32, 8, 128), ([600], [1029], 1, 1, 70), ([64], [520], 33, 1, 128)])
+def test_many_query_rows(q_lens, lens, Hq, H, D, dtype):
+    """Sequences of so many query rows that their tokens are laid out for the tensor core ahead, cut (the first ones) and not."""
+    inputs, *got = run(q_lens, lens, Hq, H, D, dtype=dtype, seed=len(lens), more_rows=2, more_tokens=100)
+    check(inputs, *got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_query_rows_out_of_range(dtype):
+    """Bad lengths, pages and a number of tokens that is too small: those sequences are left out and counted, the others are as they were."""
+    lens = [300] * 4
+    cache, table, _ = paged(lens, 1, 128, 9)
+    q = torch.randn(4 * 200, 4, 128, generator=torch.Generator().manual_seed(0)).to(dtype)
+    cu = torch.arange(0, 801, 200, dtype=torch.int32)
+    attn = TurboQuantPagedAttention(4, 128, 0.1, 1)
+
+    def call(lens=lens, table=table, total=1200):
+        before = _cabi.state_fault_counts()[0]
+        out = attn.cross(q.to(DEV), cu.to(DEV), cache.to(DEV), table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), total).cpu()
+        return out, _cabi.state_fault_counts()[0] - before
+    good, faults = call()
+    assert faults == 0
+    out, faults = call(lens=[300, -1, 10 ** 9, 300])
+    assert faults == 2 and torch.equal(out[:200], good[:200]) and not out[200:600].any() and torch.equal(out[600:], good[600:])
+    out, faults = call(total=384)                          # 3 + 4 tiles: two sequences of three
+    assert faults == 2 and torch.equal(out[:400], good[:400]) and not out[400:].any()
+    bad = table.clone()
+    bad[1, 2] = cache.shape[1]
+    out, faults = call(table=bad)
+    assert faults >= 1 and torch.equal(out[:200], good[:200]) and torch.equal(out[400:], good[400:])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("Hq, H, D", [(8, 8, 96), (5, 1, 128), (7, 1, 128), (16, 2, 65), (24, 2, 128), (3, 3, 100), (129, 1, 128)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_geometries(Hq, H, D, dtype):
@@ -173,8 +209,8 @@ def test_nan_and_infinite_queries_reach_their_rows_alone(dtype):
 
 @pytest.mark.gpu
 def test_repeats_exactly_and_reads_nothing_behind_a_sequence():
-    """Other contents behind the sequences' ends (slots, tables) and another size of the workspace: the same bits."""
-    cache, table, lens = paged([300, 200], 2, 128, 4)
+    """Other contents behind the sequences' ends (slots, tables): the same bits."""
+    cache, table, lens = paged([300, 200], 2, 128, 4, width=40)
     q = torch.randn(200, 8, 128, generator=torch.Generator().manual_seed(0)).half()
     cu = torch.tensor([0, 100, 200], dtype=torch.int32)
     attn = TurboQuantPagedAttention(8, 128, 0.1, 2)
@@ -183,10 +219,9 @@ def test_repeats_exactly_and_reads_nothing_behind_a_sequence():
     for b, n in enumerate(lens.tolist()):
         for t in range(n, (n + 15) // 16 * 16):
             other[:, table[b, t // 16], t % 16] = 0xff
-    wide = torch.full((2, 40), 10 ** 9, dtype=torch.int32)
-    wide[:, :table.shape[1]] = table
-    wide[1, 13:] = -5
-    c = attn.cross(q.to(DEV), cu.to(DEV), other.to(DEV), wide.to(DEV), lens.to(DEV), 4000)
+    table[0, 19:] = 10 ** 9
+    table[1, 13:] = -5
+    c = attn.cross(q.to(DEV), cu.to(DEV), other.to(DEV), table.to(DEV), lens.to(DEV), 500)
     assert torch.equal(a, c)
 
 

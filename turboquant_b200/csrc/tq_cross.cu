@@ -4,25 +4,34 @@
 //   out[t, h] = sum_j softmax_j(q[t, h] . k[j] * scale) v[j],      j over the tokens of the cache, t over the query rows of the sequence
 //
 // Queries and cached rows stay in the rotated domain (K^ = H S K, V^ = H S V): a query is rotated once, an output row is rotated back
-// once, and what is between is two matrix products.  With hundreds of query rows those bound it, 4 x 128 operations for each row and
-// token, and a cached row would be dequantized again for every 256 query rows; so a first kernel does that once.
+// once, and what is between is two matrix products.  A block takes one or two tiles of 128 query rows of one KV head (the query heads that share
+// it are rows too: row r is query r / G, head r % G) and a range of the tokens, 128 at a time:
 //
-//   lay out   K^ and V^ of 128 tokens and one head, and 128 rotated query rows of one head, become the two 32 KB shared-memory images that the
-//             tensor core reads (rows of 128 bytes, 16-byte pieces swizzled by the row, V^ transposed), so that the second kernel
-//             brings a tile with one contiguous bulk copy and needs no tensor map.  The query heads that share a KV head are rows of
-//             one tile: row r is query r / G, head r % G.
-//   attend    A block takes 256 query rows (two tiles) of one head and a range of the tokens.  Two warpgroups own a tile each, a thread a
-//             row; one warp copies tiles into a ring, one issues S = Q K^^T and O += P V^.  S and then P (fp16, in the same columns) of a
-//             tile and its O are all of tensor memory: 2 x (128 + 128) columns.  While one tile's row maxima and exponentials are worked
-//             out, the tensor core works for the other tile.  The running maximum is raised only when a logit exceeds it by 2^8, which
-//             makes rescaling O rare; a row needs no other thread but its own.
-//   join      Where few rows have long sequences, the tokens are cut over several blocks, whose rows a third kernel joins.
+//   two warps     bring the slots of K and V into shared memory, 64 tokens at a time (a tiled tensor copy of 16 rows a page), another fetches the norms,
+//   four warps    look the K codes up into the 32 KB image that the tensor core reads (rows of 128 bytes, 16-byte pieces swizzled by the row), four
+//                 others the V codes into its transpose, nibbles of two tokens zipped into bytes,
+//   a warp        issues S = Q K^^T and O += P V^,
+//   two warpgroups, a thread a row, take S from tensor memory, keep a running maximum and sum, and put P (fp16) into the same columns.
+//
+// Where many query rows share a sequence's tokens (prompts), a first kernel writes the images of K, V and the queries to memory once and a block only copies
+// them in, 32 KB each: the look-ups of four warps a team take longer than the products they feed (845 us looked up, 645 laid out ahead, at four sequences of 2048
+// queries on 4096 tokens, 32 heads on 8).  With few rows that would write and read 512 bytes for every 80-byte slot, and the slots are looked up as they come
+// (404 us laid out ahead, 177 looked up, at two sequences of 16 queries on 65536 tokens, 64 heads on 8).
+//
+// S, then P, and O of two tiles are all of tensor memory: 2 x (128 + 128) columns.  With two tiles of query rows each warpgroup has one, and while it works out
+// exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn, and the
+// first joins the second's sums to its own at the end.  The running maximum is raised only when a logit exceeds it by 2^8, which makes
+// rescaling O rare; a row needs no other thread but its own.  At the end O, as two fp16 parts, goes through the tensor core once more, against the Hadamard matrix
+// and the signs (exact in fp16), which brings its rows back from the rotation and its columns into order.  The code that runs once a block is kept short:
+// straight through 64 values in registers, fetched anew by every block, the butterflies took as long as ten tiles.  Where few rows have long sequences the tokens are cut over several blocks as well, whose
+// rows a second kernel joins.
 //
 // Numbers are fp16 in the tensor core with fp32 sums, brought into fp16's range by powers of two: a query row by its largest element, the norms of
 // K and V by the largest of the tile.
 //   16-bit results of 8 bits (bf16): norms are multiplied into K^ and V^, one rounding (2^-12) each.
 //   results of 11 bits and more (fp16, fp32): K^ and V^ are bare levels, scaled so that the eight of them lie within 4e-5 of fp16 values;
-//             norms multiply S and P in fp32, and a query is two fp16 parts (half again as many operations in the tensor core): what is rounded is P.
+//             norms multiply S and P in fp32, and a query is two fp16 parts (half again as many operations in the tensor core, and one
+//             tile of query rows a block): what is rounded is P.
 #include <cmath>
 #include <cstring>
 
@@ -33,31 +42,35 @@ namespace tq {
 
 constexpr int kCrossTile = 128;                      // tokens, query rows, padded head size
 constexpr int kCrossImage = kCrossTile * kCrossTile * 2;
-constexpr int kCrossThreads = 384;                   // two softmax warpgroups, and one of a copying, an issuing and two idle warps
+constexpr int kCrossTeam = 4;                        // warps that look up K, and as many for V
+constexpr int kCrossRowThreads = 384, kCrossThreads = kCrossRowThreads + 2 * kCrossTeam * 32;      // two warpgroups of rows, one of copies, norms and products; the teams
+constexpr int kCrossLaid = 2;                         // blocks of query rows a sequence from which on the images are laid out ahead
 constexpr float kCrossRaise = 8.0f;                  // P up to 2^8
 constexpr double kCrossLevelScale = 1.42803;         // see tq_scored.cu
 constexpr float kCrossNoNorm = -1000.0f;             // the logarithm of V's scale in a tile whose V is all zero
 constexpr uint32_t kCrossWaitLimit = 1u << 18, kCrossSuspendNs = 1000;
 
 struct CrossParams {
-    SplitParams f;              // what split_load_row / split_finish take: types, head size, signs, out, the cache
+    SplitParams f;              // what split_load_row / split_finish take: types, head size, signs, out, the cache; its tensor map (boxes of 16 slots)
     const int32_t* cu_q;        // [batch + 1]
-    uint8_t* kv_images;         // [tile][head][K, V][32 KB]
-    float2* tile_scales;        // [tile][head]: powers of two that the norms were divided by, K and V (their logarithm)
-    float* tile_norms;          // exact: [tile][head][K, V][128]
+    // where the images are laid out ahead:
+    uint8_t* kv_images;         // [tile][head][K, V][32 KB]; behind the last, the matrix of the way back
+    uint8_t* turn_image;
+    float2* tile_scales;        // [tile][head]: K's power of two, the logarithm of V's
+    uint16_t* tile_norms;       // exact: [tile][head][K, V][128]
     uint8_t* q_images;          // [query tile][head][part][32 KB]
     float* q_scales;            // [query tile][head][128], times the scale of the logits (base 2)
+    int64_t kv_room, q_room;    // tiles that there is room for
     float* partial_o;           // [split][query row][query head][128], rotated domain
     float* partial_lse;
-    int64_t kv_room, q_room;    // tiles that the workspace holds
-    int total_q, splits, heads;
+    int total_q, splits;
     uint16_t level_h[16];
 };
 
 static __device__ int32_t g_cross_faults = 0;
 
 struct CrossSeq {
-    int b, local;               // the sequence, and which of its tiles (pairs of query tiles) the index is
+    int b, local;               // the sequence, and which of its items the index is
     int len, qlen;              // tokens, query rows (tokens of the prompt)
     int kv0, q0;                // its first tiles
 };
@@ -72,11 +85,11 @@ __device__ __forceinline__ int cross_qlen(const CrossParams& p, int b, bool& bad
     bad = c0 < 0 || c1 < c0 || c1 > p.total_q;
     return bad ? 0 : c1 - c0;
 }
-// The sequence that item `index` of a kind belongs to (0: tiles of tokens, 1: tiles of query rows, 2: pairs of these); false: there are not so many.  A
-// sequence without queries has no tiles of tokens; one whose tiles the workspace does not hold has no tokens (or queries).  A whole warp.
+// The sequence that item `index` of a kind belongs to (0: tiles of tokens; 1, 2: that many tiles of query rows); false: there are not so many.  A sequence
+// without queries has no tiles of tokens; one that ends behind the tiles which the caller's number of tokens makes has no tokens.  A whole warp.
 template <int KIND>
 __device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, int lane, CrossSeq& s, int* faults = nullptr) {
-    int64_t kv = 0, q = 0, pairs = 0;
+    int64_t kv = 0, q = 0, items = 0;
     for (int base = 0; base < p.f.batch; base += 32) {
         int len = 0, qlen = 0, kt = 0, qt = 0;
         if (base + lane < p.f.batch) {
@@ -87,21 +100,20 @@ __device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, 
             kt = qlen > 0 ? (len + kCrossTile - 1) / kCrossTile : 0;
             if (faults) *faults += bad_len + bad_q;
         }
-        int kt_to = kt, qt_to = qt, pair_to = (qt + 1) / 2;
+        const int mine = KIND == 0 ? kt : (qt + KIND - 1) / (KIND == 0 ? 1 : KIND);
+        int kt_to = kt, qt_to = qt, to = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, kt_to, o), c = __shfl_up_sync(0xffffffffu, qt_to, o), d = __shfl_up_sync(0xffffffffu, pair_to, o);
-            if (lane >= o) { kt_to += a; qt_to += c; pair_to += d; }
+            const int a = __shfl_up_sync(0xffffffffu, kt_to, o), c = __shfl_up_sync(0xffffffffu, qt_to, o), d = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) { kt_to += a; qt_to += c; to += d; }
         }
         const bool kv_fits = kv + kt_to <= p.kv_room, q_fits = q + qt_to <= p.q_room;
         if (faults) *faults += (kt > 0 && !kv_fits) + (qt > 0 && !q_fits);
-        const int mine = KIND == 0 ? kt : KIND == 1 ? qt : (qt + 1) / 2;
-        const int64_t end = KIND == 0 ? kv + kt_to : KIND == 1 ? q + qt_to : pairs + pair_to;
-        const uint32_t hit = __ballot_sync(0xffffffffu, index < end);
+        const uint32_t hit = __ballot_sync(0xffffffffu, index < items + to);
         if (hit) {
             const int l = __ffs(hit) - 1;
             s.b = base + l;
-            s.local = (int)(index - (__shfl_sync(0xffffffffu, end, l) - __shfl_sync(0xffffffffu, mine, l)));
+            s.local = (int)(index - items) - __shfl_sync(0xffffffffu, to - mine, l);
             s.len = __shfl_sync(0xffffffffu, kv_fits ? len : 0, l);
             s.qlen = __shfl_sync(0xffffffffu, q_fits ? qlen : 0, l);
             s.kv0 = (int)(kv + __shfl_sync(0xffffffffu, kt_to - kt, l));
@@ -110,7 +122,7 @@ __device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, 
         }
         kv += __shfl_sync(0xffffffffu, kt_to, 31);
         q += __shfl_sync(0xffffffffu, qt_to, 31);
-        pairs += __shfl_sync(0xffffffffu, pair_to, 31);
+        items += __shfl_sync(0xffffffffu, to, 31);
     }
     return false;
 }
@@ -131,6 +143,25 @@ __device__ __forceinline__ int cross_exponent(float v, int to) {
 }
 __device__ __forceinline__ float cross_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
+// Where the largest norm of a tile goes, as an exponent of two.  In the images: products with levels up to 4 stay inside fp16.  Under P (exact): P is up to 2^9, and
+// an earlier tile's scale may be 2^6 behind.
+constexpr int kCrossInImage = 6, kCrossUnderP = -1;
+
+// Piece c (eight columns) of row dim of the matrix of the way back: column 16 d + w is dim 8 w + d of O.
+__device__ __forceinline__ uint4 cross_turn(int dim, int c, bool negative) {
+    const uint32_t same = (uint32_t)__popc(dim & (64 * (c & 1) + (c >> 1))) ^ (uint32_t)negative;      // d = c / 2, w = 8 (c % 2) + ...
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t a = (same ^ (uint32_t)__popc((dim >> 3) & (2 * e))) & 1u, b = (same ^ (uint32_t)__popc((dim >> 3) & (2 * e + 1))) & 1u;
+        v[e] = 0x3C003C00u | a << 15 | b << 31;
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// ---------------------------------------------------------------------------------------------
+// images laid out ahead
+// ---------------------------------------------------------------------------------------------
 constexpr int kLayThreads = 256, kLayPitch = 17;      // words of a staged V row (16 and one, for the banks)
 template <bool EXACT>
 __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid_constant__ CrossParams p) {
@@ -148,6 +179,10 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
         int faults = 0;
         cross_find<0>(p, (int64_t)1 << 60, lane, s, &faults);
         if (faults) atomicAdd(&g_cross_faults, faults);
+    }
+    if (blockIdx.x == gridDim.x - 1) {                // the matrix of the way back
+        for (int i = tid; i < kCrossTile * 16; i += kLayThreads)
+            *reinterpret_cast<uint4*>(p.turn_image + cross_piece(i >> 4, i & 15)) = cross_turn(i >> 4, i & 15, p.f.signs[i >> 4] < 0.0f);
     }
     __syncthreads();
 
@@ -189,27 +224,20 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
         }
         const int which = tid >> 7, t = tid & 127;
         const float norm = t < n ? __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(p.f.kv_cache + which * slab + slot_s[t] + kHeadDim / 2))) : 0.0f;
-        float most = fabsf(norm) < INFINITY ? fabsf(norm) : 0.0f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(norm) < INFINITY ? fabsf(norm) : 0.0f)));
         if (lane == 0) most_s[which][warp & 3] = most;
         __syncthreads();
-        // norms to [64, 128): with levels up to 4 the products stay inside fp16, and so do their sums' terms
         most = fmaxf(fmaxf(most_s[which][0], most_s[which][1]), fmaxf(most_s[which][2], most_s[which][3]));
-        const bool has = most > 0.0f;
-        const int by = cross_exponent(most, 6);
-        norm_s[which][t] = __half_as_ushort(__float2half_rn(norm * cross_power(by)));
-        if constexpr (EXACT) p.tile_norms[((tile * H + h) * 2 + which) * kCrossTile + t] = norm * cross_power(by);
-        if (t == 0) {
-            float* const to = reinterpret_cast<float*>(p.tile_scales + tile * H + h) + which;
-            *to = !which ? cross_power(-by) : has ? (float)-by : kCrossNoNorm;
-        }
+        const int by = cross_exponent(most, EXACT ? kCrossUnderP : kCrossInImage);
+        if constexpr (EXACT) p.tile_norms[((tile * H + h) * 2 + which) * kCrossTile + t] = __half_as_ushort(__float2half_rn(norm));      // as they are
+        else norm_s[which][t] = __half_as_ushort(__float2half_rn(norm * cross_power(by)));
+        if (t == 0) reinterpret_cast<float*>(p.tile_scales + tile * H + h)[which] = which ? most > 0.0f ? (float)-by : kCrossNoNorm : EXACT ? 1.0f : cross_power(-by);
         __syncthreads();
         uint8_t* const image = p.kv_images + (tile * H + h) * 2 * kCrossImage;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int r = (i & 3) * 32 + warp * 4 + (lane >> 3), c = (i >> 2) * 8 + (lane & 7);
-            const uint32_t w = k_code[i], nn = (uint32_t)norm_s[0][r] * 0x10001u;
+            const uint32_t w = k_code[i], nn = EXACT ? 0u : (uint32_t)norm_s[0][r] * 0x10001u;
             uint32_t v[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {             // dims in pairs {odd, even}, as the queries have them
@@ -218,7 +246,7 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
             }
             *reinterpret_cast<uint4*>(image + cross_piece(r, c)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
-        // V^ transposed: a lane takes eight tokens (one piece) of eight dims (one code word); nibbles of two tokens are zipped into bytes
+        // V^ transposed, dim 8 w + d as row 16 d + w: a lane takes eight tokens (one piece) of eight dims (one code word); nibbles of two tokens are zipped into bytes
         {
             const int c = (lane & 7) + 8 * (warp & 1), word = (lane >> 3) + 4 * (warp >> 1);     // pieces 0 ... 15, words 0 ... 15
             uint32_t out[8][4];
@@ -226,7 +254,7 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
             for (int pr = 0; pr < 4; pr++) {
                 const uint32_t a = codes_s[(8 * c + 2 * pr) * kLayPitch + word], b = codes_s[(8 * c + 2 * pr + 1) * kLayPitch + word];
                 const uint32_t odd = (a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u), even = ((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u);
-                const uint32_t nn = *reinterpret_cast<const uint32_t*>(&norm_s[1][8 * c + 2 * pr]);
+                const uint32_t nn = EXACT ? 0u : *reinterpret_cast<const uint32_t*>(&norm_s[1][8 * c + 2 * pr]);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     out[2 * j][pr] = level2((even >> (8 * j)) & 255u);
@@ -238,7 +266,7 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
                 }
             }
 #pragma unroll
-            for (int d = 0; d < 8; d++) *reinterpret_cast<uint4*>(image + kCrossImage + cross_piece(8 * word + d, c)) = make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
+            for (int d = 0; d < 8; d++) *reinterpret_cast<uint4*>(image + kCrossImage + cross_piece(16 * d + word, c)) = make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
         }
         __syncthreads();
     }
@@ -283,8 +311,7 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
                 v[i] *= p.f.scale;
                 top = fmaxf(top, fabsf(v[i]));
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
             const int by = cross_exponent(top, 9);    // to [512, 1024)
             const float f = p.f.k_scale < 0.0f ? -cross_power(by) : cross_power(by);
             if (lane == 0) p.q_scales[(tile * H + h) * kCrossTile + r] = fabsf(p.f.k_scale) * cross_power(-by);
@@ -304,32 +331,19 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
 // ---------------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------------
-template <bool EXACT>
-struct CrossShape {
-    static constexpr int kParts = EXACT ? 2 : 1;
-    static constexpr int kSlots = EXACT ? 3 : 5;                           // of the ring: K, V, K, V, ... of the tiles in turn
-    static constexpr uint32_t kQ = 0, kRing = 2 * kParts * kCrossImage;
-    // Norms of a tile travel with its K into one of two buffers.  The copy of K (j + 2) waits for the slot of V (j) at the latest, which is free
-    // when both warpgroups have handed over P (j), and so have read the norms of tile j.
-    static constexpr uint32_t kNorms = kRing + kSlots * kCrossImage, kNormBytes = EXACT ? 2 * kCrossTile * 4 : 0;
-    static constexpr uint32_t kBars = kNorms + 2 * kNormBytes;
-    static constexpr size_t kSmem = kBars + 256;
-    static_assert(!EXACT || kSlots <= 3, "the norms' buffers");
-    static_assert(kSmem <= 232448, "shared memory of a block");
-};
-
 // SW128, K-major: rows of 128 bytes, eight rows 1024 bytes on
-__device__ __forceinline__ uint64_t cross_desc(uint32_t addr) {
+__host__ __device__ constexpr uint64_t cross_desc(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)64 << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 // A wait of a whole warp that ends early when another role has given up.
 __device__ __forceinline__ bool cross_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
     bool done = false;
-    for (uint32_t i = 0; i < kCrossWaitLimit && !done && !*gone; i++) {
+    for (uint32_t i = 0; i < kCrossWaitLimit && !done; i++) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok) : "r"(bar), "r"(parity), "r"(kCrossSuspendNs) : "memory");
         done = ok != 0;
+        if ((i & 15) == 15 && *gone) break;
     }
     return __all_sync(0xffffffffu, done);
 }
@@ -340,6 +354,26 @@ __device__ __forceinline__ void cross_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void cross_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// Stores that keep their order among themselves and to the barriers, and loads of what does not change (the table), which have none: the compiler is
+// free to look codes up ahead of the stores of those before.
+__device__ __forceinline__ void cross_sts(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d));
+}
+__device__ __forceinline__ uint32_t cross_table(uint32_t at) {
+    uint32_t v;
+    asm("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float4 cross_lds_f4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float2 cross_lds_f2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+    return v;
 }
 // 32 columns of the thread's tensor-memory lane; the values are there after cross_ld_wait of the same registers.
 __device__ __forceinline__ void cross_ld(uint32_t taddr, float* r) {
@@ -352,6 +386,16 @@ __device__ __forceinline__ void cross_ld(uint32_t taddr, float* r) {
           "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void cross_ld16(uint32_t taddr, float* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+                   "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]) : "r"(taddr));
+}
+__device__ __forceinline__ void cross_ld_wait16(float* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]) :: "memory");
+}
 __device__ __forceinline__ void cross_ld_wait(float* r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
@@ -359,6 +403,13 @@ __device__ __forceinline__ void cross_ld_wait(float* r) {
                    "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]),
                    "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
                  :: "memory");
+}
+__device__ __forceinline__ void cross_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
 }
 __device__ __forceinline__ void cross_st(uint32_t taddr, const uint32_t* r) {
     asm volatile(
@@ -371,148 +422,581 @@ __device__ __forceinline__ void cross_st(uint32_t taddr, const uint32_t* r) {
         : "memory");
 }
 
-template <bool EXACT>
-__global__ void __launch_bounds__(kCrossThreads, 1) cross_attend_kernel(const __grid_constant__ CrossParams p) {
-    using F = CrossShape<EXACT>;
+// Shared memory as absolute addresses of the block's window, whose first 1024 bytes are the system's.  Where the block looks codes up itself: two rings of slots,
+// K's and V's, of three halves of a tile (64 tokens); barriers and small words; the table at a multiple of its size (a shift and one logic
+// instruction make an entry's address); the images on their 1024-byte boundaries; the norms.  Where the images come laid out: barriers, images, norms.
+constexpr int kCrossHalf = kCrossTile / 2, kCrossUnit = kCrossHalf * kSlotBytes, kCrossStages = 3, kCrossMetas = 4;
+constexpr uint32_t kCrossRaw = 1024;                                     // K's ring, then V's
+constexpr uint32_t kCrossLut = 32768;                                    // entry v, column lane: {level(v & 15), level(v >> 4)}
+template <bool EXACT, bool LAID>
+struct CrossMap {
+    static constexpr uint32_t kBars = LAID ? 1024 : kCrossRaw + 2 * kCrossStages * kCrossUnit;
+    static constexpr uint32_t kScales = kBars + 512;                     // of tile t at t % kCrossMetas: K's power of two, the logarithm of V's
+    static constexpr uint32_t kSigns = kScales + kCrossMetas * 8;        // a bit a dim: negative
+    static constexpr uint32_t kQ = LAID ? 2048 : 65536;                  // two images: tiles of query rows, or the two parts of one
+    // Images in turn, of K and V.  Two tiles of query rows: K0 V0 K1 V1 ... ; one: K0 K1 V0 K2 V1 ... , the order in which they are needed.  Behind the last comes
+    // the matrix of the way back, where the next K would be.  Looked up here each is written as two halves (64 tokens); it is free when its product has been formed.
+    static constexpr int kImages = LAID ? 5 : 3;
+    static constexpr uint32_t kImg = kQ + 2 * kCrossImage;               // (before the first: the query rows as they come)
+    // The norms of tile t at t % 4: for the rows (exact), fp16, K's and V's; or for the look-ups, fp16, K's twice each.  When S (t - 2) has been formed P (t - 4)
+    // has been handed over, so nobody reads the norms of tile t - 4 any more.
+    static constexpr uint32_t kNorms = kImg + kImages * kCrossImage;
+    static constexpr uint32_t kQScale = kNorms;                          // (before the first norms)
+    static constexpr int kNormBytes = EXACT ? 2 * kCrossTile * 2 : LAID ? 0 : 2 * kCrossTile * 4;
+    static constexpr uint32_t kNormsEnd = kNorms + (kCrossMetas * kNormBytes > kCrossTile * 16 ? kCrossMetas * kNormBytes : kCrossTile * 16);      // (behind the last: sums of a group)
+    static constexpr size_t kSmem = kNormsEnd - 1024;
+    static_assert(kSigns + 16 <= (LAID ? kQ : kCrossLut) && kSmem <= 232448 && kCrossUnit % 128 == 0, "shared memory of a block");
+};
+
+// The exponent that brings the largest of a tile's norms (four a lane) to [2^to, 2^(to + 1)).
+__device__ __forceinline__ int cross_norm_exponent(const float (&norm)[4], int to, bool& has) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (fabsf(norm[i]) < INFINITY) most = fmaxf(most, fabsf(norm[i]));
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));      // bits of numbers that are not negative sort as they do
+    has = most > 0.0f;
+    return cross_exponent(most, to);
+}
+
+// LAID: the images are there, laid out by the kernel before this one; else the codes are looked up and the queries rotated here.
+template <bool EXACT, bool LAID>
+__global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cross_attend_kernel(const __grid_constant__ CrossParams p) {
+    constexpr int kTiles = EXACT ? 1 : 2;             // of query rows
+    using M = CrossMap<EXACT, LAID>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, H = p.f.kv_heads, G = p.f.real_group;
-    const uint32_t base = smem_u32(smem);
+    uint8_t* const window = smem - smem_u32(smem);    // address 0 of the block's window
     grid_launch_dependents();
-    if (base & 1023) {                                // the swizzle counts on it
+    if (smem_u32(smem) != 1024) {                     // the map counts on it
         grid_dependency_wait();
         if (tid == 0 && blockIdx.x == 0) atomicAdd(&g_cross_faults, 1);
         return;
     }
-    // barriers of 8 bytes: Q, the ring's full and empty, S and P and O of the two tiles; then the tensor-memory address and the flag of a role that gave up
-    const uint32_t bars = base + F::kBars;
-    const uint32_t q_full = bars, ring_full = bars + 8, ring_empty = ring_full + 8 * F::kSlots, s_full = ring_empty + 8 * F::kSlots, p_full = s_full + 16,
-                   o_full = p_full + 16, drained = o_full + 16;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + F::kBars + 192);
-    volatile int* const gone = reinterpret_cast<volatile int*>(smem + F::kBars + 196);
-    if (tid == 0) {
-        cross_bar_init(q_full, 1);
-        for (int i = 0; i < F::kSlots; i++) {
-            cross_bar_init(ring_full + 8 * i, 1);
-            cross_bar_init(ring_empty + 8 * i, 1);
+    const uint32_t bars = M::kBars;
+    const uint32_t raw_full = bars, raw_empty = raw_full + 16 * kCrossStages, meta_full = raw_empty + 16 * kCrossStages, s_formed = meta_full + 8 * kCrossMetas,
+                   img_full = s_formed + 8 * kCrossMetas, img_empty = img_full + 16 * M::kImages, s_full = img_empty + 8 * M::kImages, p_full = s_full + 16,
+                   o_full = p_full + 16, a_full = o_full + 16, d_full = a_full + 16, drained = d_full + 16;      // raw: K's stages, then V's; images: two halves
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(window + M::kBars + 400);
+    volatile int* const gone = reinterpret_cast<volatile int*>(window + M::kBars + 404);
+    if (tid == 9 * 32) {
+        for (int i = 0; i < 2 * kCrossStages; i++) {
+            cross_bar_init(raw_full + 8 * i, 1);
+            cross_bar_init(raw_empty + 8 * i, kCrossTeam);
+        }
+        for (int i = 0; i < kCrossMetas; i++) {
+            cross_bar_init(meta_full + 8 * i, 1);
+            cross_bar_init(s_formed + 8 * i, 1);
+        }
+        for (int i = 0; i < M::kImages; i++) {
+            cross_bar_init(img_full + 16 * i, kCrossTeam);
+            cross_bar_init(img_full + 16 * i + 8, LAID ? 1 : kCrossTeam);
+            cross_bar_init(img_empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
             cross_bar_init(s_full + 8 * i, 1);
-            cross_bar_init(p_full + 8 * i, 4);        // the warps of the tile
+            cross_bar_init(p_full + 8 * i, 4);        // the warps of a group
             cross_bar_init(o_full + 8 * i, 1);
+            cross_bar_init(a_full + 8 * i, 4);
+            cross_bar_init(d_full + 8 * i, 1);
         }
         cross_bar_init(drained, 1);
         *gone = 0;
         fence_barrier_init();
     }
+    if (!LAID && warp >= 12) {                        // the table, ahead of the wait
+        const uint32_t mine = p.level_h[lane & 15];
+        for (int v = 4 * (warp - 12) + (lane >> 3); v < 256; v += 8 * kCrossTeam) {
+            const uint32_t e = __shfl_sync(0xffffffffu, mine, v & 15) | (__shfl_sync(0xffffffffu, mine, v >> 4) << 16);
+            *reinterpret_cast<uint4*>(window + kCrossLut + v * 128 + 16 * (lane & 7)) = make_uint4(e, e, e, e);
+        }
+    }
     grid_dependency_wait();
+    if (!LAID && blockIdx.x == 0 && warp == 8) {      // what is left out is counted once
+        CrossSeq none;
+        int faults = 0;
+        cross_find<0>(p, (int64_t)1 << 60, lane, none, &faults);
+        if (faults) atomicAdd(&g_cross_faults, faults);
+    }
+    if (!LAID && warp == 13) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t negative = __ballot_sync(0xffffffffu, p.f.signs[32 * i + lane] < 0.0f);
+            if (lane == 0) reinterpret_cast<uint32_t*>(window + M::kSigns)[i] = negative;
+        }
+    }
     CrossSeq s;
     const int64_t item = blockIdx.x / p.splits;
     const int split = (int)(blockIdx.x - item * p.splits), h = (int)(item % H);
-    if (!cross_find<2>(p, item / H, lane, s) || s.qlen == 0) return;      // uniform over the block
-    const int rows = s.qlen * G, qt = (rows + kCrossTile - 1) / kCrossTile, q_tile = 2 * s.local, both = q_tile + 1 < qt ? 2 : 1;
+    if (!cross_find<kTiles>(p, item / H, lane, s) || s.qlen == 0) return; // uniform over the block
+    const int rows = s.qlen * G, row0 = s.local * kTiles * kCrossTile;
+    const bool solo = kTiles == 1 || rows - row0 <= kCrossTile;           // one tile of query rows
     const int all = (s.len + kCrossTile - 1) / kCrossTile;
     const int j0 = (int)((int64_t)all * split / p.splits), n = (int)((int64_t)all * (split + 1) / p.splits) - j0;      // the block's tiles of tokens
+
     if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + F::kBars + 192), "r"(512));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(M::kBars + 400), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    const int pages = (s.len + kPageTokens - 1) / kPageTokens, page0 = j0 * (kCrossTile / kPageTokens);
+    bool bad_page = false;
+    auto page_id = [&](int i) -> int {                // page i of the block's range; none and bad ones: page 0
+        if (page0 + i >= pages) return 0;
+        const int id = p.f.page_indices[(int64_t)s.b * p.f.max_pages + page0 + i];
+        const bool good = (uint64_t)(int64_t)id < (uint64_t)p.f.num_blocks;
+        bad_page |= !good;
+        return good ? id : 0;
+    };
+    const int units = 2 * n;                          // halves of tiles
+    // Item numbers of the images, see M::kImages.
+    auto k_item = [&](int t) { return solo ? (t < 2 ? t : 2 * t - 1) : 2 * t; };
+    auto v_item = [&](int t) { return solo ? 2 * t + 2 : 2 * t + 1; };
+
+    const int D = p.f.head_dim;
+    // K's and V's first slots: there is room.  ids: pages of eight units, and of the next eight.
+    const int which = warp == 11, ring8 = which * kCrossStages;
+    int id_now = 0, id_next = 0;
+    auto copy_unit = [&](int u) {                     // lanes 0 ... 3 a page each
+        const int stage = u % kCrossStages, id = __shfl_sync(0xffffffffu, id_now, (4 * (u & 7) + lane) & 31), some = max(0, min(4, pages - page0 - 4 * u));
+        const uint32_t bar = raw_full + 8 * (ring8 + stage);
+        if (lane == 0) split_expect(bar, (uint32_t)(some * kPageTokens * kSlotBytes));
+        __syncwarp();
+        if (lane < some)
+            split_box(kCrossRaw + (ring8 + stage) * kCrossUnit + lane * kPageTokens * kSlotBytes, &p.f.cache_map, h * kSlotBytes, id * kPageTokens, which, bar);
+    };
+    if constexpr (!LAID) {
+        // Query rows, as they come, into shared memory: 16-bit rows of whole pieces of 16 bytes by asynchronous copies, all in flight together.
+        const int q_rows = min(rows - row0, solo ? kCrossTile : 2 * kCrossTile), q_first = p.cu_q[s.b];
+        const bool plain = p.f.q_dtype != TQ_F32 && D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f.q) & 15) == 0;
+        auto row_of = [&](int r) -> int64_t {             // of the query tensor
+            const int row = row0 + r, qi = row / G;
+            return (int64_t)(q_first + qi) * p.f.real_heads + h * G + (row - qi * G);
+        };
+        if (plain) {
+            const int pieces = D / 8;
+            for (int i = tid; i < q_rows * pieces; i += kCrossThreads) {
+                const int r = i / pieces, c = i - r * pieces;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(M::kImg + r * 256 + 16 * c), "l"(reinterpret_cast<const uint16_t*>(p.f.q) + row_of(r) * D + 8 * c) : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        __syncthreads();
+        if (warp == 8 || warp == 11) {
+            id_now = page_id(lane);
+            id_next = page_id(32 + lane);
+            for (int u = 0; u < min(units, kCrossStages); u++) copy_unit(u);
+        }
+        // Rotated, by a power of two to [512, 1024), into the images.  Sixteen warps take rows warp, warp + 16, ... , two at a time.
+        if (warp < 8 || warp >= 12) {
+            const float4 sign = reinterpret_cast<const float4*>(p.f.signs)[lane];
+#pragma unroll 1
+            for (int r0 = warp < 8 ? warp : warp - 4; r0 < (solo ? kCrossTile : 2 * kCrossTile); r0 += 2 * 16) {
+                float v[2][4], top[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int r = r0 + 16 * u;
+                    const bool in = r < q_rows && 4 * lane < D;
+                    if (!plain) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[u][i] = in && 4 * lane + i < D ? load_q(p.f.q, p.f.q_dtype, row_of(r) * D + 4 * lane + i) : 0.0f;
+                    } else {
+                        const uint2 raw = in ? lds64(M::kImg + r * 256 + 8 * lane) : make_uint2(0u, 0u);
+                        if (p.f.q_dtype == TQ_BF16) {
+                            v[u][0] = __uint_as_float(raw.x << 16); v[u][1] = __uint_as_float(raw.x & 0xffff0000u);
+                            v[u][2] = __uint_as_float(raw.y << 16); v[u][3] = __uint_as_float(raw.y & 0xffff0000u);
+                        } else {
+                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+                            v[u][0] = a.x; v[u][1] = a.y; v[u][2] = b.x; v[u][3] = b.y;
+                        }
+                    }
+                    v[u][0] *= sign.x; v[u][1] *= sign.y; v[u][2] *= sign.z; v[u][3] *= sign.w;
+                    split_fwht<4>(v[u], lane);
+                    top[u] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        v[u][i] *= p.f.scale;
+                        top[u] = fmaxf(top[u], fabsf(v[u][i]));
+                    }
+                    top[u] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top[u])));
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int r = r0 + 16 * u, by = cross_exponent(top[u], 9);
+                    const float f = p.f.k_scale < 0.0f ? -cross_power(by) : cross_power(by);
+                    if (lane == 0) reinterpret_cast<float*>(window + M::kQScale)[r] = fabsf(p.f.k_scale) * cross_power(-by);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[u][i] *= f;
+                    uint8_t* const to = window + M::kQ + (r >> 7) * kCrossImage + cross_piece(r & 127, lane >> 1) + 8 * (lane & 1);
+                    const uint32_t a = pack_half2(v[u][1], v[u][0]), b = pack_half2(v[u][3], v[u][2]);      // pairs {odd, even}, as the codes have them
+                    *reinterpret_cast<uint2*>(to) = make_uint2(a, b);
+                    if constexpr (EXACT) {
+                        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
+                        *reinterpret_cast<uint2*>(to + kCrossImage) = make_uint2(pack_half2(v[u][1] - fa.x, v[u][0] - fa.y), pack_half2(v[u][3] - fb.x, v[u][2] - fb.y));
+                    }
+                }
+            }
+            fence_proxy_async();
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;                 // S / P of tile i at 128 i, O at 256 + 128 i
-    const int64_t kv_at = (int64_t)(s.kv0 + j0) * H + h;      // image of the block's tile j: kv_at + j H
+    const uint32_t tmem = *tmem_slot;                 // S / P of group i at 128 i, O at 256 + 128 i; all 512 columns: zero
+    const int64_t q_unit = (int64_t)(s.q0 + s.local * kTiles) * H + h;                    // the block's query images: this, and H on
+    float q_scale = 0.0f;
+    if constexpr (LAID) {
+        if (warp < 8) q_scale = p.q_scales[(q_unit + (solo ? 0 : (warp >> 2) * H)) * kCrossTile + (tid & 127)];
+    } else {
+        if (warp < 8) q_scale = reinterpret_cast<const float*>(window + M::kQScale)[(solo ? 0 : (warp >> 2) * kCrossTile) + (tid & 127)];
+        __syncthreads();                              // the scales' place is the norms' from here on
+    }
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 8) {
-            // =============================== copies ======================================================
-            if (n > 0 && lane == 0) {
-                split_expect(q_full, both * F::kParts * kCrossImage);
-                for (int i = 0; i < both; i++)
-                    for (int a = 0; a < F::kParts; a++)
-                        cross_copy(base + F::kQ + (i * F::kParts + a) * kCrossImage,
-                                   p.q_images + (((int64_t)(s.q0 + q_tile + i) * H + h) * F::kParts + a) * kCrossImage, kCrossImage, q_full);
+    if (!LAID && warp >= 12) {
+        const uint32_t lut_lane = kCrossLut + 4 * lane;
+        // byte j of a word through the table: 128 bytes an entry
+        auto level2 = [&](uint32_t w, int j) { return cross_table(((j == 0 ? w << 7 : w >> (8 * j - 7)) & 0x7f80u) | lut_lane); };
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const bool on_k = warp < 12 + kCrossTeam;
+        const int mate = on_k ? warp - 12 : warp - 12 - kCrossTeam;
+        bool ok = true;
+        int stage = 0, turn = 0;
+        const uint32_t ring = on_k ? 0 : kCrossStages;      // of the barriers and stages: K's first
+        for (int u = 0; u < units && ok; u++) {
+            const int t = u >> 1, half = u & 1;
+            const uint32_t raw = kCrossRaw + (ring + stage) * kCrossUnit, norms = M::kNorms + (uint32_t)(t % kCrossMetas) * M::kNormBytes;
+            ok = cross_wait(raw_full + 8 * (ring + stage), turn, gone);
+            if (!EXACT && half == 0) ok = ok && cross_wait(meta_full + 8 * (t % kCrossMetas), (t / kCrossMetas) & 1, gone);
+            const int item = on_k ? k_item(t) : v_item(t), slot = item % M::kImages;
+            if (half == 0) ok = ok && cross_wait(img_empty + 8 * slot, ((item / M::kImages) & 1) ^ 1, gone);
+            if (!ok) break;
+            const uint32_t image = M::kImg + slot * kCrossImage;
+            if (on_k) {
+                // =========================== K ================================================================
+                // A lane takes 16 code bytes of a row, eight lanes the same of eight rows: no bank is met twice, at 80 bytes a row or in the image.
+                // Both rows are looked up before either is stored: the assembler keeps loads and stores of shared memory in order.
+                const int q = lane >> 3, r0 = 8 * mate + (lane & 7);
+                constexpr int kStep = 8 * kCrossTeam, kRows = kCrossHalf / kStep;
+                uint32_t v[kRows][16], nn[kRows];
+                uint4 code[kRows];
+#pragma unroll
+                for (int i = 0; i < kRows; i++) {
+                    code[i] = lds128(raw + (kStep * i + r0) * kSlotBytes + 16 * q);
+                    if constexpr (!EXACT) nn[i] = lds32(norms + 4 * (kCrossHalf * half + kStep * i + r0));
+                }
+#pragma unroll
+                for (int i = 0; i < kRows; i++) {
+                    const uint32_t w4[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+#pragma unroll
+                    for (int e = 0; e < 16; e++) v[i][e] = level2(w4[e >> 2], e & 3);
+                }
+#pragma unroll
+                for (int i = 0; i < kRows; i++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        if constexpr (!EXACT) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) v[i][4 * c + j] = cross_mul2(v[i][4 * c + j], nn[i]);
+                        }
+                        cross_sts(image + cross_piece(kCrossHalf * half + kStep * i + r0, 4 * q + c), v[i][4 * c], v[i][4 * c + 1], v[i][4 * c + 2], v[i][4 * c + 3]);
+                    }
+            } else {
+                // =========================== V ================================================================
+                // A lane takes eight tokens (a piece of the image's rows) of a code word (eight dims); dim 8 w + d is row 16 d + w of the image, so that
+                // neighbouring lanes store to rows of different swizzle.
+                const int w = lane & 15, c = 2 * mate + (lane >> 4);      // piece of the half
+                const uint32_t at = raw + 8 * c * kSlotBytes + 4 * w;
+                uint32_t code[8], nn[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; e++) code[e] = lds32(at + e * kSlotBytes);
+                if constexpr (!EXACT) {
+                    const uint4 v = lds128(norms + 4 * kCrossTile + 2 * (kCrossHalf * half + 8 * c));
+                    nn[0] = v.x; nn[1] = v.y; nn[2] = v.z; nn[3] = v.w;
+                }
+                // odd and even dims of token pairs, in place of the codes
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const uint32_t a = code[e], b = code[e + 1];
+                    code[e] = ((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u);
+                    code[e + 1] = (a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u);
+                }
+#pragma unroll
+                for (int j2 = 0; j2 < 4; j2 += 2) {
+                    uint32_t out[2][2][4];
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            out[j][0][e] = level2(code[2 * e], j2 + j);
+                            out[j][1][e] = level2(code[2 * e + 1], j2 + j);
+                        }
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int d = 0; d < 2; d++) {
+                            uint32_t (&o)[4] = out[j][d];
+                            if constexpr (!EXACT) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[e] = cross_mul2(o[e], nn[e]);
+                            }
+                            cross_sts(image + cross_piece(16 * (2 * (j2 + j) + d) + w, 8 * half + c), o[0], o[1], o[2], o[3]);
+                        }
+                }
             }
-            int k = 0, slot = 0, parity = 1;          // of the wait for an empty slot: free at first
-            for (; k < 2 * n; k++) {
-                if (!cross_wait(ring_empty + 8 * slot, parity, gone)) break;
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                cross_arrive(raw_empty + 8 * (ring + stage));
+                cross_arrive(img_full + 16 * slot + 8 * half);
+            }
+            if (++stage == kCrossStages) {
+                stage = 0;
+                turn ^= 1;
+            }
+        }
+        if (on_k && ok && n > 0 && p.splits == 1) {
+            // =============================== the matrix of the way back ======================================
+            const int item = k_item(n), slot = item % M::kImages;
+            ok = cross_wait(img_empty + 8 * slot, ((item / M::kImages) & 1) ^ 1, gone);
+            if (ok) {
+#pragma unroll 1
+                for (int i = tid - 12 * 32; i < kCrossTile * 16; i += kCrossTeam * 32) {
+                    const uint4 v = cross_turn(i >> 4, i & 15, (lds32(M::kSigns + 4 * (i >> 9)) >> ((i >> 4) & 31)) & 1u);
+                    cross_sts(M::kImg + slot * kCrossImage + cross_piece(i >> 4, i & 15), v.x, v.y, v.z, v.w);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) cross_arrive(img_full + 16 * slot + 8);
+            }
+        }
+        if (!ok) *gone = 1;
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (LAID && warp == 8) {
+            // =============================== copies: queries, images ======================================
+            constexpr int kParts = EXACT ? 2 : 1;
+            const int items = n == 0 ? 0 : solo || p.splits == 1 ? 2 * n + 1 : 2 * n;
+            int k = 0;
+            if (lane == 0 && n > 0) {
+                const int q_images = solo ? kParts : 2;
+                split_expect(raw_full, (uint32_t)(q_images * kCrossImage));
+                for (int a = 0; a < q_images; a++) cross_copy(M::kQ + a * kCrossImage, p.q_images + ((q_unit + (EXACT ? 0 : a) * H) * kParts + (EXACT ? a : 0)) * kCrossImage, kCrossImage, raw_full);
+            }
+            for (; k < items; k++) {
+                const int slot = k % M::kImages, v = solo ? k > 0 && !(k & 1) : k & 1, t = solo ? v ? (k >> 1) - 1 : (k + 1) >> 1 : k >> 1;      // item k is V (t) or K (t)
+                if (t == n && p.splits > 1) continue;
+                if (!cross_wait(img_empty + 8 * slot, ((k / M::kImages) & 1) ^ 1, gone)) break;
                 if (lane == 0) {
-                    const int64_t image = kv_at + (int64_t)(k >> 1) * H;
-                    const uint32_t bar = ring_full + 8 * slot, more = (k & 1) == 0 ? F::kNormBytes : 0;
-                    split_expect(bar, kCrossImage + more);
-                    cross_copy(base + F::kRing + slot * kCrossImage, p.kv_images + (image * 2 + (k & 1)) * kCrossImage, kCrossImage, bar);
-                    if (more) cross_copy(base + F::kNorms + ((k >> 1) & 1) * F::kNormBytes, p.tile_norms + image * 2 * kCrossTile, F::kNormBytes, bar);
+                    const uint8_t* const from = t == n ? p.turn_image : p.kv_images + (((int64_t)(s.kv0 + j0 + t) * H + h) * 2 + v) * kCrossImage;
+                    split_expect(img_full + 16 * slot + 8, kCrossImage);
+                    cross_copy(M::kImg + slot * kCrossImage, from, kCrossImage, img_full + 16 * slot + 8);
                 }
                 __syncwarp();
-                if (++slot == F::kSlots) {
-                    slot = 0;
-                    parity ^= 1;
-                }
             }
-            if (k < 2 * n) {                          // gave up: what is in flight gets its time to land
+            if (k < items) {                          // gave up: what is in flight gets its time to land
                 if (lane == 0) atomicAdd(&g_cross_faults, 1);
                 *gone = 1;
-                for (int i = k > F::kSlots ? k - F::kSlots : 0; i < k; i++)
-                    for (uint32_t w = 0; w < kCrossWaitLimit / 64; w++)
-                        if (split_try_wait(ring_full + 8 * (i % F::kSlots), (i / F::kSlots) & 1)) break;
                 for (uint32_t w = 0; w < kCrossWaitLimit / 64; w++)
-                    if (split_try_wait(q_full, 0)) break;
+                    if (split_try_wait(raw_full, 0)) break;
+                for (int c = k > M::kImages ? k - M::kImages : 0; c < k; c++)
+                    for (uint32_t w = 0; w < kCrossWaitLimit / 64; w++)
+                        if (split_try_wait(img_full + 16 * (c % M::kImages) + 8, (c / M::kImages) & 1)) break;
             }
+        } else if (LAID && warp == 10) {
+            // =============================== norms and scales ============================================
+            const int64_t unit0 = (int64_t)(s.kv0 + j0) * H + h;
+            float2 scales = make_float2(0.0f, 0.0f);
+            uint4 norms = make_uint4(0u, 0u, 0u, 0u);
+            auto fetch = [&](int t) {
+                if (t >= n) return;
+                scales = p.tile_scales[unit0 + (int64_t)t * H];
+                if constexpr (EXACT) norms = reinterpret_cast<const uint4*>(p.tile_norms + (unit0 + (int64_t)t * H) * 2 * kCrossTile)[lane];
+            };
+            fetch(0);
+            bool ok = true;
+            for (int t = 0; t < n && ok; t++) {
+                const int slot = t % kCrossMetas;
+                if (t >= kCrossMetas) ok = cross_wait(s_formed + 8 * ((t - 2) % kCrossMetas), ((t - 2) / kCrossMetas) & 1, gone);
+                if (!ok) break;
+                if constexpr (EXACT) *reinterpret_cast<uint4*>(window + M::kNorms + slot * M::kNormBytes + 16 * lane) = norms;
+                if (lane == 0) reinterpret_cast<float2*>(window + M::kScales)[slot] = scales;
+                fetch(t + 1);
+                __syncwarp();
+                if (lane == 0) cross_arrive(meta_full + 8 * slot);
+            }
+            if (!ok) *gone = 1;
+        } else if (!LAID && (warp == 8 || warp == 11)) {
+            // =============================== copies: K, V ================================================
+            int u = min(units, kCrossStages);
+            for (; u < units; u++) {
+                if ((u & 7) == 0) {
+                    id_now = id_next;
+                    id_next = page_id(4 * u + 32 + lane);
+                }
+                if (!cross_wait(raw_empty + 8 * (ring8 + u % kCrossStages), ((u / kCrossStages) & 1) ^ 1, gone)) break;
+                copy_unit(u);
+            }
+            if (bad_page && which == 0) atomicAdd(&g_cross_faults, 1);
+            if (u < units) {                          // gave up: what is in flight gets its time to land
+                if (lane == 0) atomicAdd(&g_cross_faults, 1);
+                *gone = 1;
+                for (int k = u > kCrossStages ? u - kCrossStages : 0; k < u; k++)
+                    for (uint32_t w = 0; w < kCrossWaitLimit / 64; w++)
+                        if (split_try_wait(raw_full + 8 * (ring8 + k % kCrossStages), (k / kCrossStages) & 1)) break;
+            }
+        } else if (!LAID && warp == 10) {
+            // =============================== norms =======================================================
+            // Lane l has tokens l, l + 32, l + 64, l + 96; those of the next tile and the pages of the one after are on their way.
+            const int64_t slab = p.f.num_blocks * kPageTokens * H * kSlotBytes;
+            int ids[4];
+            uint16_t nk[4], nv[4];
+            auto fetch_ids = [&](int t) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) ids[e] = t < n ? page_id(8 * t + 2 * e + (lane >> 4)) : 0;
+            };
+            auto fetch = [&](int t) {
+                const int valid = t < n ? s.len - (j0 + t) * kCrossTile : 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint8_t* const at = p.f.kv_cache + (((int64_t)ids[e] * kPageTokens + (lane & 15)) * H + h) * kSlotBytes + kHeadDim / 2;
+                    const bool in = lane + 32 * e < valid;
+                    nk[e] = in ? *reinterpret_cast<const uint16_t*>(at) : (uint16_t)0;
+                    nv[e] = in ? *reinterpret_cast<const uint16_t*>(at + slab) : (uint16_t)0;
+                }
+            };
+            fetch_ids(0);
+            fetch(0);
+            fetch_ids(1);
+            bool ok = true;
+            for (int t = 0; t < n && ok; t++) {
+                const int slot = t % kCrossMetas;
+                float fk[4], fv[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    fk[e] = __half2float(__ushort_as_half(nk[e]));
+                    fv[e] = __half2float(__ushort_as_half(nv[e]));
+                }
+                fetch(t + 1);
+                fetch_ids(t + 2);
+                if (t >= kCrossMetas) ok = cross_wait(s_formed + 8 * ((t - 2) % kCrossMetas), ((t - 2) / kCrossMetas) & 1, gone);
+                if (!ok) break;
+                bool has_k, has_v;
+                const int by_k = cross_norm_exponent(fk, kCrossInImage, has_k), by_v = cross_norm_exponent(fv, EXACT ? kCrossUnderP : kCrossInImage, has_v);
+                const float sk = cross_power(by_k), sv = cross_power(by_v);
+                uint8_t* const to = window + M::kNorms + slot * M::kNormBytes;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int tok = lane + 32 * e;
+                    if constexpr (EXACT) {
+                        reinterpret_cast<__half*>(to)[tok] = __float2half_rn(fk[e]);      // as they are: the powers of two are part of the exponents
+                        reinterpret_cast<__half*>(to)[kCrossTile + tok] = __float2half_rn(fv[e]);
+                    } else {
+                        reinterpret_cast<uint32_t*>(to)[tok] = pack_half2(fk[e] * sk, fk[e] * sk);
+                        reinterpret_cast<__half*>(to + 4 * kCrossTile)[tok] = __float2half_rn(fv[e] * sv);
+                    }
+                }
+                if (lane == 0) reinterpret_cast<float2*>(window + M::kScales)[slot] = make_float2(EXACT ? 1.0f : cross_power(-by_k), has_v ? (float)-by_v : kCrossNoNorm);
+                __syncwarp();
+                if (lane == 0) cross_arrive(meta_full + 8 * slot);
+            }
+            if (!ok) *gone = 1;
         } else if (warp == 9 && n > 0) {
             // =============================== matrix products ==============================================
             constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kCrossTile >> 3) << 17) | ((uint32_t)(kCrossTile >> 4) << 24);      // fp16 x fp16 -> fp32, 128 x 128
-            bool ok = cross_wait(q_full, 0, gone);
-            int slot = 0, parity = 0;
-            auto next_slot = [&] {
-                if (++slot == F::kSlots) {
-                    slot = 0;
-                    parity ^= 1;
-                }
-            };
-            auto scores = [&](int i) {                // S of tile i from the K image in the slot
-                const uint64_t b0 = cross_desc(base + F::kRing + slot * kCrossImage);
+            const uint64_t q_desc = cross_desc(M::kQ), img_desc = cross_desc(M::kImg);
+            constexpr uint64_t kImage16 = kCrossImage / 16;
+            auto scores = [&](int i, int slot) {      // S of group i from the K in a slot
+                const uint64_t k_desc = img_desc + (uint64_t)slot * kImage16, a_desc = q_desc + (EXACT || solo ? 0 : i) * kImage16;
 #pragma unroll
-                for (int a = 0; a < F::kParts; a++) {
-                    const uint64_t a0 = cross_desc(base + F::kQ + (i * F::kParts + a) * kCrossImage);
+                for (int a = 0; a < (EXACT ? 2 : 1); a++)
 #pragma unroll
                     for (int kk = 0; kk < 8; kk++) {
                         const uint64_t off = (uint64_t)((kk >> 2) * 1024 + (kk & 3) * 2);      // 16 dims on, in units of 16 bytes
-                        mq_mma(tmem + 128 * i, a0 + off, b0 + off, idesc, a || kk ? 1u : 0u);
+                        mq_mma(128 * i, a_desc + a * kImage16 + off, k_desc + off, idesc, a || kk ? 1u : 0u);
                     }
-                }
                 cross_commit(s_full + 8 * i);
             };
-            if (ok) ok = cross_wait(ring_full, 0, gone);
-            tc_fence_after();
-            if (ok && elect_one()) {
-                for (int i = 0; i < both; i++) scores(i);
-                cross_commit(ring_empty);
+            auto formed = [&](int t) {                // S (t) of all groups
+                cross_commit(img_empty + 8 * (k_item(t) % M::kImages));
+                cross_commit(s_formed + 8 * (t % kCrossMetas));
+            };
+            auto values = [&](int i, int slot, int half, bool more) {      // O of group i += P V of 64 tokens
+                const uint64_t v_desc = img_desc + (uint64_t)slot * kImage16 + (uint64_t)(half * 1024);
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++) mq_mma_ts(256 + 128 * i, 128 * i + 32 * half + 8 * kk, v_desc + (uint64_t)(kk * 2), idesc, more || half || kk ? 1u : 0u);
+            };
+            auto image_there = [&](int item, int half) { return cross_wait(img_full + 16 * (item % M::kImages) + (LAID ? 8 : 8 * half), (item / M::kImages) & 1, gone); };
+            bool ok = !LAID || cross_wait(raw_full, 0, gone);      // the queries
+            // Two tiles of query rows: step u is group u % 2 and tile u / 2 of the tokens; one: group u % 2, tile u.  After P V of a step comes the next S
+            // of its group.
+            const int first = solo ? min(2, n) : 1, steps = solo ? n : 2 * n;
+            for (int t = 0; t < first && ok; t++) {
+                ok = image_there(k_item(t), 0) && image_there(k_item(t), 1);
+                tc_fence_after();
+                if (ok && elect_one()) {
+                    scores(solo ? t : 0, k_item(t) % M::kImages);
+                    if (!solo) scores(1, k_item(0) % M::kImages);
+                    formed(t);
+                }
+                __syncwarp();
             }
-            __syncwarp();
-            next_slot();
-            for (int j = 0; j < n && ok; j++) {
-                const int v_slot = slot, v_parity = parity;
-                next_slot();
-                ok = cross_wait(ring_full + 8 * v_slot, v_parity, gone);
-                const bool more = j + 1 < n;
-                if (ok && more) ok = cross_wait(ring_full + 8 * slot, parity, gone);
-                for (int i = 0; i < both && ok; i++) {
-                    ok = cross_wait(p_full + 8 * i, j & 1, gone);
+            for (int u = 0; u < steps && ok; u++) {
+                const int i = u & 1, t = solo ? u : u >> 1, next = t + (solo ? 2 : 1), k = u >> 1;
+                const bool last = solo || i == 1;     // group of this tile
+                const bool fresh = solo || i == 0;    // images that this step is the first to read
+                if constexpr (LAID) {                 // they are there before P is: one wait between P and the products
+                    ok = !fresh || (image_there(v_item(t), 1) && (next >= n || image_there(k_item(next), 1)));
+                    ok = ok && cross_wait(p_full + 8 * i, k & 1, gone);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t b0 = cross_desc(base + F::kRing + v_slot * kCrossImage);
+                        values(i, v_item(t) % M::kImages, 0, k > 0);
+                        values(i, v_item(t) % M::kImages, 1, true);
+                        if (last) cross_commit(img_empty + 8 * (v_item(t) % M::kImages));
+                        if (next >= n) cross_commit(o_full + 8 * i);
+                        else scores(i, k_item(next) % M::kImages);
+                        if (next < n && last) formed(next);
+                    }
+                    __syncwarp();
+                    continue;
+                }
+                ok = cross_wait(p_full + 8 * i, k & 1, gone);
 #pragma unroll
-                        for (int kk = 0; kk < 8; kk++)
-                            mq_mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * kk, b0 + (uint64_t)((kk >> 2) * 1024 + (kk & 3) * 2), idesc, j || kk ? 1u : 0u);
-                        if (i == both - 1) cross_commit(ring_empty + 8 * v_slot);
-                        if (more) scores(i);
-                        else cross_commit(o_full + 8 * i);
-                        if (more && i == both - 1) cross_commit(ring_empty + 8 * slot);
+                for (int half = 0; half < 2; half++) {
+                    if (fresh) ok = ok && image_there(v_item(t), half);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        values(i, v_item(t) % M::kImages, half, k > 0);
+                        if (half == 1 && last) cross_commit(img_empty + 8 * (v_item(t) % M::kImages));
+                        if (half == 1 && next >= n) cross_commit(o_full + 8 * i);
                     }
                     __syncwarp();
                 }
-                next_slot();
+                if (!ok) break;
+                if (next < n) {
+                    if (fresh) ok = image_there(k_item(next), 0) && image_there(k_item(next), 1);
+                    tc_fence_after();
+                    if (ok && elect_one()) {
+                        scores(i, k_item(next) % M::kImages);
+                        if (last) formed(next);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (ok && p.splits == 1) {                // the way back: the two parts of O's rows, in S's place, against the matrix in V's
+                ok = image_there(k_item(n), 1);
+                for (int i = 0; i < (solo ? 1 : 2) && ok; i++) {
+                    ok = cross_wait(a_full + 8 * i, 0, gone);
+                    tc_fence_after();
+                    if (ok && elect_one()) {
+                        const uint64_t turn = cross_desc(M::kImg + (uint32_t)(k_item(n) % M::kImages) * kCrossImage);
+#pragma unroll 1
+                        for (int kk = 0; kk < 16; kk++)
+                            mq_mma_ts(256 + 128 * i, 128 * i + 8 * kk, turn + (uint64_t)(((kk >> 2) & 1) * 1024 + (kk & 3) * 2), idesc, kk ? 1u : 0u);
+                        cross_commit(d_full + 8 * i);
+                    }
+                    __syncwarp();
+                }
             }
             if (!ok) {
                 if (lane == 0 && !*gone) atomicAdd(&g_cross_faults, 1);
@@ -525,88 +1009,142 @@ __global__ void __launch_bounds__(kCrossThreads, 1) cross_attend_kernel(const __
         }
     } else {
         // =============================== a row a thread ===================================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int i = warp >> 2, r = tid & 127, row = (q_tile + i) * kCrossTile + r;
+        // A row of S is read 32 columns at a time: kept in registers it would take more than the 128 a thread that leave the look-ups theirs, and there is no
+        // first-level cache to speak of behind this much shared memory for what spills.
+        if constexpr (LAID) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        const int i = warp >> 2, r = tid & 127, row = row0 + (solo ? 0 : i * kCrossTile) + r;
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tm_s = tmem + 128 * i + lane_at, tm_o = tmem + 256 + 128 * i + lane_at;
         bool ok = true;
-        float m = kNoMax, l = 0.0f, x[128];
-        float ev_most = -1000.0f;
-        const bool mine = i < both;
-        const float q_scale = mine ? p.q_scales[((int64_t)(s.q0 + q_tile + i) * H + h) * kCrossTile + r] : 0.0f;
-        // The scale of V that the sums are kept in: the largest of the block's tiles.
-        for (int j = lane; j < n; j += 32) ev_most = fmaxf(ev_most, p.tile_scales[kv_at + (int64_t)j * H].y);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ev_most = fmaxf(ev_most, __shfl_xor_sync(0xffffffffu, ev_most, o));
-        float2 scales = n > 0 ? p.tile_scales[kv_at] : make_float2(0.0f, 0.0f);
-        for (int j = 0; j < n && mine && ok; j++) {
-            // A masked logit is -inf times kf: kf is no zero (a scale of zero).  A tile whose V is zero, or as good as that beside the largest, has P
-            // scaled by 2^-60: out of fp16, not out of the row's sum.
-            const float kf = fmaxf(scales.x * q_scale, 1e-36f), dv = fmaxf(scales.y - ev_most, -60.0f);
-            if (j + 1 < n) scales = p.tile_scales[kv_at + (int64_t)(j + 1) * H];
-            ok = cross_wait(s_full + 8 * i, j & 1, gone);
+        float m = kNoMax, l = 0.0f, ev_ref = kCrossNoNorm;
+        const int turns = solo ? (n + 1 - i) >> 1 : n;
+        for (int k = 0; k < turns && ok; k++) {
+            const int t = solo ? 2 * k + i : k;
+            ok = cross_wait(meta_full + 8 * (t % kCrossMetas), (t / kCrossMetas) & 1, gone) && cross_wait(s_full + 8 * i, k & 1, gone);
             if (!ok) break;
             tc_fence_after();
+            const uint32_t norms = M::kNorms + (uint32_t)(t % kCrossMetas) * M::kNormBytes;
+            const float2 scales = cross_lds_f2(M::kScales + 8 * (t % kCrossMetas));
+            // A masked logit is -inf times kf: kf is no zero (a scale of zero).
+            const float kf = fmaxf(scales.x * q_scale, 1e-36f), ev = scales.y;
+            const int valid = s.len - (j0 + t) * kCrossTile;
+            const P2 kf2 = pk(kf, kf);
+            // P is scaled by 2^dv: a tile whose V is zero, or as good as that beside others, by 2^-60, out of fp16 but not out of the row's sum.  Where the norms
+            // multiply P as they are, dv is that of the sums alone.
+            auto shift = [&] { return EXACT ? fminf(fmaxf(-ev_ref, -60.0f), 60.0f) : fmaxf(ev - ev_ref, -60.0f); };
+            float dv = shift();
+            // Norms of eight tokens, fp16 as in the cache (a broadcast load costs a wavefront for every four bytes: half of what fp32 ones would).
+            auto times_norms = [&](int which, int col, float* v) {
+                const uint4 a = lds128(norms + 2 * (kCrossTile * which + col));
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int c = 0; c < 4; c++) cross_ld(tm_s + 32 * c, x + 32 * c);
+                for (int e = 0; e < 4; e++) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                    v[2 * e] *= f.x;
+                    v[2 * e + 1] *= f.y;
+                }
+            };
+            // exp2 of 16 columns into fp16 pairs, and their sum
+            auto exponentials = [&](int col, float* v, P2 sub, P2& sum, uint32_t* ph) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) cross_ld_wait(x + 32 * c);
-            const float* const norms = reinterpret_cast<const float*>(smem + F::kNorms + (j & 1) * F::kNormBytes);
-            if constexpr (EXACT) {
+                for (int e = 0; e < 16; e += 2) {
+                    up(fma2(pk(v[e], v[e + 1]), kf2, sub), v[e], v[e + 1]);
+                    v[e] = fast_exp2(v[e]);
+                    v[e + 1] = fast_exp2(v[e + 1]);
+                    sum = add2(sum, pk(v[e], v[e + 1]));
+                }
+                if constexpr (EXACT) {
 #pragma unroll
-                for (int c = 0; c < 128; c += 4) {
-                    const float4 t = *reinterpret_cast<const float4*>(norms + c);
-                    x[c] *= t.x; x[c + 1] *= t.y; x[c + 2] *= t.z; x[c + 3] *= t.w;
+                    for (int e = 0; e < 16; e += 8) times_norms(1, col + e, v + e);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) ph[e >> 1] = pack_half2(v[e], v[e + 1]);
+            };
+            P2 sum = pk(0.0f, 0.0f);
+            bool done = false;
+            // In the common case the running maximum needs no look at the row: P is worked out from the maximum that there is, and its sum tells whether any of it
+            // is too large (2^9; NaN and infinity too).  P waits in registers until the warp knows, as it takes the place of S.
+            if (valid >= kCrossTile && ev <= ev_ref + 6.0f) {
+                const P2 sub = pk(dv - m, dv - m);
+                const float most = 512.0f * fast_exp2(dv);
+                uint32_t ph[64];
+                float v[2][16];                       // the next columns are on their way
+                cross_ld16(tm_s, v[0]);
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    cross_ld_wait16(v[c & 1]);
+                    if (c < 7) cross_ld16(tm_s + 16 * (c + 1), v[(c + 1) & 1]);
+                    if constexpr (EXACT) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 8) times_norms(0, 16 * c + e, v[c & 1] + e);
+                    }
+                    exponentials(16 * c, v[c & 1], sub, sum, ph + 8 * c);
+                }
+                float sa, sb;
+                up(sum, sa, sb);
+                done = __all_sync(0xffffffffu, sa + sb <= most);
+                if (done) {
+                    cross_st(tm_s, ph);
+                    cross_st(tm_s + 32, ph + 32);
                 }
             }
-            const int valid = s.len - (j0 + j) * kCrossTile;
-            if (valid < kCrossTile) {                 // the last tile of the sequence
+            if (!done) {
+                // The maximum first, then P, 32 columns at a time: the columns of P (c) are those of S (c / 2), read already.
+                auto columns = [&](int c, float (&v)[32]) {      // S of 32 columns, as it counts
+                    cross_ld(tm_s + 32 * c, v);
+                    cross_ld_wait(v);
+                    if constexpr (EXACT) {
 #pragma unroll
-                for (int c = 0; c < 128; c++)
-                    if (c >= valid) x[c] = -INFINITY;
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        for (int e = 0; e < 32; e += 8) times_norms(0, 32 * c + e, v + e);
+                    }
+                    if (valid < 32 * c + 32) {        // the last tile of the sequence
 #pragma unroll
-            for (int c = 0; c < 128; c += 4) {
-                mx[0] = fmaxf(mx[0], x[c]); mx[1] = fmaxf(mx[1], x[c + 1]); mx[2] = fmaxf(mx[2], x[c + 2]); mx[3] = fmaxf(mx[3], x[c + 3]);
-            }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kf;      // kf >= 0
-            const bool raise = top > m + kCrossRaise;
-            if (__any_sync(0xffffffffu, raise)) {
-                const float c = raise ? fast_exp2(m - top) : 1.0f;
-                if (raise) m = top;
-                l *= c;
-                if (j > 0) {                          // S (j) is there, so the products before it are done with O
+                        for (int e = 0; e < 32; e++)
+                            if (32 * c + e >= valid) v[e] = -INFINITY;
+                    }
+                };
+                float v[32], top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    columns(c, v);
 #pragma unroll
-                    for (int a = 0; a < 4; a++) {
-                        float o[32];
-                        cross_ld(tm_o + 32 * a, o);
-                        cross_ld_wait(o);
+                    for (int e = 0; e < 32; e++) top = fmaxf(top, v[e]);
+                }
+                top *= kf;                            // kf > 0
+                const bool raise = top > m + kCrossRaise;
+                // The power of two of V that the sums are kept in is the first tile's, until a tile's is 2^6 above it.
+                if (__any_sync(0xffffffffu, raise) || ev > ev_ref + 6.0f) {
+                    float c = raise ? fast_exp2(m - top) : 1.0f;
+                    if (raise) m = top;
+                    l *= c;
+                    if (ev > ev_ref + 6.0f) {
+                        c *= fast_exp2(ev_ref - ev);
+                        ev_ref = ev;
+                    }
+                    if (k > 0) {                      // S is there, so the products before it are done with O
+#pragma unroll 1
+                        for (int a = 0; a < 4; a++) {
+                            cross_ld(tm_o + 32 * a, v);
+                            cross_ld_wait(v);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] *= c;
-                        cross_st(tm_o + 32 * a, reinterpret_cast<const uint32_t*>(o));
+                            for (int e = 0; e < 32; e++) v[e] *= c;
+                            cross_st(tm_o + 32 * a, reinterpret_cast<const uint32_t*>(v));
+                        }
                     }
                 }
-            }
-            const P2 kf2 = pk(kf, kf), sub = pk(dv - m, dv - m);
-            P2 sum = pk(0.0f, 0.0f);
-            uint32_t ph[64];
-#pragma unroll
-            for (int c = 0; c < 128; c += 2) {
-                float a, b;
-                up(fma2(pk(x[c], x[c + 1]), kf2, sub), a, b);
-                a = fast_exp2(a);
-                b = fast_exp2(b);
-                sum = add2(sum, pk(a, b));
-                if constexpr (EXACT) {
-                    const float2 t = *reinterpret_cast<const float2*>(norms + kCrossTile + c);
-                    a *= t.x;
-                    b *= t.y;
+                dv = shift();
+                const P2 sub = pk(dv - m, dv - m);
+                sum = pk(0.0f, 0.0f);
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    uint32_t ph[16];
+                    columns(c, v);
+                    exponentials(32 * c, v, sub, sum, ph);
+                    exponentials(32 * c + 16, v + 16, sub, sum, ph + 8);
+                    cross_st16(tm_s + 16 * c, ph);
                 }
-                ph[c >> 1] = pack_half2(a, b);
             }
-            cross_st(tm_s, ph);
-            cross_st(tm_s + 32, ph + 32);
             float sa, sb;
             up(sum, sa, sb);
             l += (sa + sb) * fast_exp2(-dv);
@@ -615,74 +1153,145 @@ __global__ void __launch_bounds__(kCrossThreads, 1) cross_attend_kernel(const __
             __syncwarp();
             if (lane == 0) cross_arrive(p_full + 8 * i);
         }
-        // ---- the row: normalized, rotated back, out; or a partial ------------------------------------------
-        if (mine && ok && n > 0) ok = cross_wait(o_full + 8 * i, 0, gone);
-        if (mine && !ok) *gone = 1;
-        if (mine && ok) {
-            tc_fence_after();
-            if (n > 0) {
+        // ---- the row: joined, normalized, rotated back, out; or a partial ----------------------------------
+        if (ok && turns > 0) ok = cross_wait(o_full + 8 * i, 0, gone);
+        if (!ok) *gone = 1;
+        tc_fence_after();
+        // O of the row is in units of 2^ev_ref; with a second group's sums, brought over in images that are free, in units of the larger.
+        const bool joined = solo && n > 1;
+        float scale = 1.0f, scale_other = 0.0f;
+        // (the two images that are not the matrix of the way back: 64 rows each)
+        const uint32_t joint = M::kImg + (uint32_t)((k_item(n) + 1 + (r >> 6)) % M::kImages) * kCrossImage + (uint32_t)(r & 63) * kCrossTile * 4;
+        if (joined) {
+            float4* const sums = reinterpret_cast<float4*>(window + M::kNorms);
+            if (i == 1) {                             // once the first group's products are done with the images too
+                if (ok) ok = cross_wait(o_full, 0, gone);
+                if (ok) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        float v[32];
+                        cross_ld(tm_o + 32 * c, v);
+                        cross_ld_wait(v);
 #pragma unroll
-                for (int c = 0; c < 4; c++) cross_ld(tm_o + 32 * c, x + 32 * c);
-#pragma unroll
-                for (int c = 0; c < 4; c++) cross_ld_wait(x + 32 * c);
+                        for (int e = 0; e < 8; e++)
+                            cross_sts(joint + 16 * ((8 * c + e) ^ (r & 7)), __float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
+                    }
+                    sums[r] = make_float4(m, l, ev_ref, 0.0f);
+                }
             }
-            const float f = l == 0.0f ? 0.0f : p.f.v_scale * fast_exp2(ev_most) / l;
-            const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (i == 0) {
+                const float4 other = sums[r];
+                const float mm = fmaxf(m, other.x), ev = fmaxf(ev_ref, other.z), c0 = fast_exp2(m - mm), c1 = fast_exp2(other.x - mm);
+                scale = c0 * fast_exp2(ev_ref - ev);
+                scale_other = c1 * fast_exp2(other.z - ev);
+                m = mm;
+                l = l * c0 + other.y * c1;
+                ev_ref = ev;
+            }
+        }
+        if (__all_sync(0xffffffffu, ok && !(solo && i == 1) && !(joined && *gone))) {
+            const bool none = l == 0.0f, live = row < rows, cut = p.splits > 1;
+            const float inv = none ? 0.0f : 1.0f / l, lse2 = none ? -INFINITY : m + log2f(l), unit = p.f.v_scale * fast_exp2(ev_ref);
+            scale *= inv;
+            scale_other *= inv;
+            const int qi = row / G, g = row - qi * G;
+            const int64_t to = live ? (int64_t)(p.cu_q[s.b] + qi) * p.f.real_heads + h * G + g : 0, at = (int64_t)split * p.total_q * p.f.real_heads + to;
+            // The weighted mean, columns as O has them: a partial, or two fp16 parts in S's place for the way back (at most 2^15: a mean of rows of levels below 4 times
+            // norms below 2^7, under powers of two up to 2^6).
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                float v[32];
+                if (turns > 0) {
+                    cross_ld(tm_o + 32 * c, v);
+                    cross_ld_wait(v);
+                }
+                if (joined) {
 #pragma unroll
-            for (int c = 0; c < 128; c++) x[c] = l == 0.0f ? 0.0f : x[c] * f;
-            if (row < rows) {
-                const int qi = row / G, g = row - qi * G;
-                const int64_t to = (int64_t)(p.cu_q[s.b] + qi) * p.f.real_heads + h * G + g;
-                if (p.splits > 1) {
-                    const int64_t at = (int64_t)split * p.total_q * p.f.real_heads + to;
-                    float4* dst = reinterpret_cast<float4*>(p.partial_o + at * kCrossTile);
-#pragma unroll
-                    for (int c = 0; c < 32; c++) dst[c] = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
-                    p.partial_lse[at] = lse2;
+                    for (int e = 0; e < 8; e++) {
+                        const float4 o = cross_lds_f4(joint + 16 * ((8 * c + e) ^ (r & 7)));
+                        v[4 * e] = v[4 * e] * scale + o.x * scale_other; v[4 * e + 1] = v[4 * e + 1] * scale + o.y * scale_other;
+                        v[4 * e + 2] = v[4 * e + 2] * scale + o.z * scale_other; v[4 * e + 3] = v[4 * e + 3] * scale + o.w * scale_other;
+                    }
                 } else {
 #pragma unroll
-                    for (int w = 1; w < 128; w <<= 1) {
+                    for (int e = 0; e < 32; e++) v[e] *= scale;
+                }
+                if (none) {
 #pragma unroll
-                        for (int c = 0; c < 128; c++) {
-                            if ((c & w) == 0) {
-                                const float a = x[c], b = x[c + w];
-                                x[c] = a + b;
-                                x[c + w] = a - b;
-                            }
-                        }
+                    for (int e = 0; e < 32; e++) v[e] = 0.0f;
+                }
+                if (cut) {
+                    if (live) {
+                        float4* const dst = reinterpret_cast<float4*>(p.partial_o + at * kCrossTile + 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) dst[e] = make_float4(v[4 * e] * unit, v[4 * e + 1] * unit, v[4 * e + 2] * unit, v[4 * e + 3] * unit);
+                    }
+                    __syncwarp();
+                } else if (n > 0) {
+                    uint32_t a[16], b[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        a[e] = pack_half2(v[2 * e], v[2 * e + 1]);
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&a[e]));
+                        b[e] = pack_half2(v[2 * e] - back.x, v[2 * e + 1] - back.y);
+                    }
+                    cross_st16(tm_s + 16 * c, a);
+                    cross_st16(tm_s + 64 + 16 * c, b);
+                }
+            }
+            if (live) {
+                if (cut) p.partial_lse[at] = lse2;
+                else if (p.f.out_lse) p.f.out_lse[to] = lse2 * 0.6931471805599453f;
+            }
+            if (!cut) {
+                if (n > 0) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) cross_arrive(a_full + 8 * i);
+                    ok = cross_wait(d_full + 8 * i, 0, gone);
+                    tc_fence_after();
+                }
+                const bool whole = p.f.out_dtype != TQ_F32 && D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f.out) & 15) == 0;
+                const float f = unit * p.f.scale;
+#pragma unroll 1
+                for (int c = 0; c < 4 && ok; c++) {
+                    float v[32];
+                    __syncwarp();
+                    if (n > 0) {
+                        cross_ld(tm_o + 32 * c, v);
+                        cross_ld_wait(v);
                     }
 #pragma unroll
-                    for (int c = 0; c < 128; c += 4) {
-                        const float4 sg = reinterpret_cast<const float4*>(p.f.signs)[c >> 2];
-                        x[c] *= p.f.scale * sg.x; x[c + 1] *= p.f.scale * sg.y; x[c + 2] *= p.f.scale * sg.z; x[c + 3] *= p.f.scale * sg.w;
-                    }
-                    const int D = p.f.head_dim;
-                    if (p.f.out_dtype != TQ_F32 && D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f.out) & 15) == 0) {
-                        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.f.out) + to * D);
+                    for (int e = 0; e < 32; e++) v[e] = none ? 0.0f : v[e] * f;
+                    if (!live) continue;
+                    if (whole) {
+                        uint16_t* const dst = reinterpret_cast<uint16_t*>(p.f.out) + to * D + 32 * c;
 #pragma unroll
-                        for (int c = 0; c < 16; c++) {
-                            uint32_t w[4];
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t u[4];
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
+                            for (int k = 0; k < 4; k++) {
                                 if (p.f.out_dtype == TQ_BF16) {
-                                    const __nv_bfloat162 t = __floats2bfloat162_rn(x[8 * c + 2 * e], x[8 * c + 2 * e + 1]);
-                                    w[e] = *reinterpret_cast<const uint32_t*>(&t);
+                                    const __nv_bfloat162 t = __floats2bfloat162_rn(v[8 * e + 2 * k], v[8 * e + 2 * k + 1]);
+                                    u[k] = *reinterpret_cast<const uint32_t*>(&t);
                                 } else {
-                                    w[e] = pack_half2(x[8 * c + 2 * e], x[8 * c + 2 * e + 1]);
+                                    u[k] = pack_half2(v[8 * e + 2 * k], v[8 * e + 2 * k + 1]);
                                 }
                             }
-                            if (8 * c < D) dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                            if (32 * c + 8 * e < D) *reinterpret_cast<uint4*>(dst + 8 * e) = make_uint4(u[0], u[1], u[2], u[3]);
                         }
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 128; c++) {
-                            if (c >= D) continue;
-                            if (p.f.out_dtype == TQ_BF16) reinterpret_cast<__nv_bfloat16*>(p.f.out)[to * D + c] = __float2bfloat16_rn(x[c]);
-                            else if (p.f.out_dtype == TQ_F16) reinterpret_cast<__half*>(p.f.out)[to * D + c] = __float2half_rn(x[c]);
-                            else reinterpret_cast<float*>(p.f.out)[to * D + c] = x[c];
+                        for (int e = 0; e < 32; e++) {
+                            if (32 * c + e >= D) continue;
+                            const int64_t o = to * D + 32 * c + e;
+                            if (p.f.out_dtype == TQ_BF16) reinterpret_cast<__nv_bfloat16*>(p.f.out)[o] = __float2bfloat16_rn(v[e]);
+                            else if (p.f.out_dtype == TQ_F16) reinterpret_cast<__half*>(p.f.out)[o] = __float2half_rn(v[e]);
+                            else reinterpret_cast<float*>(p.f.out)[o] = v[e];
                         }
                     }
-                    if (p.f.out_lse) p.f.out_lse[to] = lse2 * 0.6931471805599453f;
                 }
             }
         }
@@ -717,8 +1326,9 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
     for (int s = 0; s < p.splits; s++) {
         const float w = fast_exp2(p.partial_lse[s * rows + at] - m);
         l += w;
-        const float4 v = *reinterpret_cast<const float4*>(p.partial_o + (s * rows + at) * kCrossTile + 4 * lane);
-        o[0] = fmaf(w, v.x, o[0]); o[1] = fmaf(w, v.y, o[1]); o[2] = fmaf(w, v.z, o[2]); o[3] = fmaf(w, v.w, o[3]);
+        const float* const v = p.partial_o + (s * rows + at) * kCrossTile + 64 * (lane & 1) + (lane >> 1);      // dim 8 w + d is column 16 d + w
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(w, v[16 * e], o[e]);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -732,6 +1342,7 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
 // host side
 // ---------------------------------------------------------------------------------------------
 int device_sm_count(int* out);
+int encode_cache_map(CUtensorMap* map, const void* kv_cache, int64_t num_blocks, int64_t row_bytes, int box_bytes, int slabs);
 
 int cross_fault_count(int32_t* out) {
     TQ_CUDA(cudaMemcpyFromSymbol(out, g_cross_faults, sizeof(int32_t)));
@@ -741,25 +1352,31 @@ int cross_fault_count(int32_t* out) {
 static size_t cross_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct CrossLayout {
-    int64_t kv_room, q_room;
+    bool laid;
+    int64_t items, kv_room, q_room;     // tiles or pairs of tiles of query rows, tiles of tokens and of query rows, at most
     int splits;
-    size_t scales, norms, q_images, q_scales, partial_lse, partial_o, end;      // the images of K and V are in front
+    size_t turn, scales, norms, q_images, q_scales, partial_lse, partial_o, end;      // the images of K and V are in front
 };
-static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, int heads, int kv_heads, int max_pages, bool exact, int sms) {
+static bool cross_exact(int out_dtype) { return out_dtype != TQ_BF16; }
+static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, int heads, int kv_heads, int max_pages, int out_dtype, int sms) {
     CrossLayout l;
-    const int64_t G = heads / kv_heads, rows = total_q * G;
-    l.kv_room = total_tokens / kCrossTile + batch;          // every sequence may end inside a tile
+    const bool exact = cross_exact(out_dtype);
+    const int64_t per = (exact ? 1 : 2) * kCrossTile, rows = (int64_t)total_q * (heads / kv_heads);
+    l.items = rows / per + batch;                           // every sequence may end inside one
+    l.kv_room = total_tokens / kCrossTile + batch;
     l.q_room = rows / kCrossTile + batch;
-    // As many cuts of the tokens as fill the SMs, of four tiles at least.
-    const int64_t pairs = (rows + 2 * kCrossTile - 1) / (2 * kCrossTile), blocks = (pairs > batch ? pairs : batch) * kv_heads;
+    l.laid = rows > kCrossLaid * per * batch;
+    // As many cuts of the tokens as fill the SMs, of two tiles (one a warpgroup) at least.
+    const int64_t some = (rows + per - 1) / per, blocks = (some > batch ? some : batch) * kv_heads;
     const int64_t longest = (int64_t)max_pages * kPageTokens < total_tokens ? (int64_t)max_pages * kPageTokens : total_tokens;
-    const int64_t most = longest / (4 * kCrossTile), fit = blocks > 0 ? sms / blocks : 1;
+    const int64_t most = (longest + 2 * kCrossTile - 1) / (2 * kCrossTile), fit = sms / blocks;
     l.splits = (int)(fit < most ? fit : most);
     if (l.splits < 1) l.splits = 1;
-    const size_t units = (size_t)l.kv_room * kv_heads, q_units = (size_t)l.q_room * kv_heads, parts = exact ? 2 : 1;
-    l.scales = units * 2 * kCrossImage;
+    const size_t units = l.laid ? (size_t)l.kv_room * kv_heads : 0, q_units = l.laid ? (size_t)l.q_room * kv_heads : 0, parts = exact ? 2 : 1;
+    l.turn = units * 2 * kCrossImage;
+    l.scales = l.turn + (l.laid ? kCrossImage : 0);
     l.norms = l.scales + cross_up(units * sizeof(float2));
-    l.q_images = l.norms + (exact ? cross_up(units * 2 * kCrossTile * 4) : 0);
+    l.q_images = l.norms + (exact ? cross_up(units * 2 * kCrossTile * 2) : 0);
     l.q_scales = l.q_images + q_units * parts * kCrossImage;
     l.partial_lse = l.q_scales + cross_up(q_units * kCrossTile * 4);
     const size_t cut = l.splits > 1 ? (size_t)l.splits * total_q * heads : 0;
@@ -767,21 +1384,22 @@ static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, in
     l.end = l.partial_o + cross_up(cut * kCrossTile * 4);
     return l;
 }
-static bool cross_exact(int out_dtype) { return out_dtype != TQ_BF16; }
 
-template <bool EXACT>
-static int launch_cross(const CrossParams& p, int sms, int64_t pairs, cudaStream_t s) {
-    using F = CrossShape<EXACT>;
+template <bool EXACT, bool LAID>
+static int launch_cross(const CrossParams& p, int sms, int64_t blocks, cudaStream_t s) {
+    constexpr size_t kSmem = CrossMap<EXACT, LAID>::kSmem;
     static bool configured[64] = {};
     int dev = 0;
     TQ_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        TQ_CUDA(cudaFuncSetAttribute(cross_attend_kernel<EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::kSmem));
+        TQ_CUDA(cudaFuncSetAttribute(cross_attend_kernel<EXACT, LAID>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const int64_t units = (p.kv_room + p.q_room) * p.f.kv_heads, lay = units < 4 * sms ? units : 4 * sms;
-    TQ_CUDA(launch_serialized(cross_lay_out_kernel<EXACT>, dim3((unsigned)lay), dim3(kLayThreads), 0, s, p));
-    TQ_CUDA(launch_serialized(cross_attend_kernel<EXACT>, dim3((unsigned)(pairs * p.f.kv_heads * p.splits)), dim3(kCrossThreads), F::kSmem, s, p));
+    if constexpr (LAID) {
+        const int64_t units = (p.kv_room + p.q_room) * p.f.kv_heads, lay = units < 4 * sms ? units : 4 * sms;
+        TQ_CUDA(launch_serialized(cross_lay_out_kernel<EXACT>, dim3((unsigned)lay), dim3(kLayThreads), 0, s, p));
+    }
+    TQ_CUDA(launch_serialized(cross_attend_kernel<EXACT, LAID>, dim3((unsigned)blocks), dim3(LAID ? kCrossRowThreads : kCrossThreads), kSmem, s, p));
     if (p.splits > 1) {
         const int64_t rows = (int64_t)p.total_q * p.f.real_heads;
         TQ_CUDA(launch_serialized(cross_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p));
@@ -794,7 +1412,7 @@ static int launch_cross(const CrossParams& p, int sms, int64_t pairs, cudaStream
 extern "C" size_t tq_cross_workspace_bytes(int batch, int total_q, int64_t total_tokens, int num_q_heads, int num_kv_heads, int max_pages, int out_dtype) {
     int sms = 0;
     if (batch < 1 || total_q < 1 || total_tokens < 0 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_pages < 1 || tq::device_sm_count(&sms) != TQ_OK) return 0;
-    return tq::cross_layout(batch, total_q, total_tokens, num_q_heads, num_kv_heads, max_pages, tq::cross_exact(out_dtype), sms).end;
+    return tq::cross_layout(batch, total_q, total_tokens, num_q_heads, num_kv_heads, max_pages, out_dtype, sms).end;
 }
 
 extern "C" int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* cu_seqlens_q, int batch, int num_q_heads, int num_kv_heads, int head_dim,
@@ -818,9 +1436,9 @@ extern "C" int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* 
     if (rc != TQ_OK) return rc;
     const bool exact = cross_exact(out_dtype);
     const int G = num_q_heads / num_kv_heads;
-    const CrossLayout l = cross_layout(batch, total_q, total_tokens, num_q_heads, num_kv_heads, max_pages, exact, sms);
-    const int64_t pairs = ((int64_t)total_q * G) / (2 * kCrossTile) + batch;
-    TQ_REQUIRE((int64_t)total_q * num_q_heads < 1ll << 31 && l.kv_room < 1 << 30 && pairs * num_kv_heads * l.splits < 1ll << 31, TQ_ERR_UNSUPPORTED,
+    const CrossLayout l = cross_layout(batch, total_q, total_tokens, num_q_heads, num_kv_heads, max_pages, out_dtype, sms);
+    const int64_t blocks = l.items * num_kv_heads * l.splits;
+    TQ_REQUIRE((int64_t)total_q * num_q_heads < 1ll << 31 && l.kv_room < 1 << 30 && blocks < 1ll << 31, TQ_ERR_UNSUPPORTED,
                "too many rows or tokens for one launch");
     TQ_REQUIRE(workspace_bytes >= l.end, TQ_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, l.end);
 
@@ -845,14 +1463,15 @@ extern "C" int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* 
     p.f.head_dim = head_dim;
     p.cu_q = cu_seqlens_q;
     p.kv_images = ws;
+    p.turn_image = ws + l.turn;
     p.tile_scales = reinterpret_cast<float2*>(ws + l.scales);
-    p.tile_norms = reinterpret_cast<float*>(ws + l.norms);
+    p.tile_norms = reinterpret_cast<uint16_t*>(ws + l.norms);
     p.q_images = ws + l.q_images;
     p.q_scales = reinterpret_cast<float*>(ws + l.q_scales);
     p.partial_lse = reinterpret_cast<float*>(ws + l.partial_lse);
-    p.partial_o = reinterpret_cast<float*>(ws + l.partial_o);
     p.kv_room = l.kv_room;
     p.q_room = l.q_room;
+    p.partial_o = reinterpret_cast<float*>(ws + l.partial_o);
     p.total_q = total_q;
     p.splits = l.splits;
     const double inv = 1.0 / std::sqrt((double)kHeadDim);
@@ -863,6 +1482,9 @@ extern "C" int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* 
     }
     p.f.v_scale = (float)(inv / kCrossLevelScale);
     p.f.k_scale = (float)(inv / kCrossLevelScale * (double)sm_scale * 1.4426950408889634);
+    rc = encode_cache_map(&p.f.cache_map, kv_cache, num_blocks, (int64_t)num_kv_heads * slot_bytes, slot_bytes, 1);
+    if (rc != TQ_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return exact ? launch_cross<true>(p, sms, pairs, s) : launch_cross<false>(p, sms, pairs, s);
+    if (l.laid) return exact ? launch_cross<true, true>(p, sms, blocks, s) : launch_cross<false, true>(p, sms, blocks, s);
+    return exact ? launch_cross<true, false>(p, sms, blocks, s) : launch_cross<false, false>(p, sms, blocks, s);
 }
