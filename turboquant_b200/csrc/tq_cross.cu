@@ -58,9 +58,7 @@ struct CrossParams {
     uint8_t* turn_image;
     float2* tile_scales;        // [tile][head]: K's power of two, the logarithm of V's
     uint16_t* tile_norms;       // exact: [tile][head][K, V][128]
-    uint8_t* q_images;          // [query tile][head][part][32 KB]
-    float* q_scales;            // [query tile][head][128], times the scale of the logits (base 2)
-    int64_t kv_room, q_room;    // tiles that there is room for
+    int64_t kv_room;            // tiles that there is room for
     float* partial_o;           // [split][query row][query head][128], rotated domain
     float* partial_lse;
     int total_q, splits;
@@ -72,7 +70,7 @@ static __device__ int32_t g_cross_faults = 0;
 struct CrossSeq {
     int b, local;               // the sequence, and which of its items the index is
     int len, qlen;              // tokens, query rows (tokens of the prompt)
-    int kv0, q0;                // its first tiles
+    int kv0;                    // its first tile of tokens
 };
 
 __device__ __forceinline__ int cross_len(const CrossParams& p, int b, bool& bad) {
@@ -89,39 +87,36 @@ __device__ __forceinline__ int cross_qlen(const CrossParams& p, int b, bool& bad
 // without queries has no tiles of tokens; one that ends behind the tiles which the caller's number of tokens makes has no tokens.  A whole warp.
 template <int KIND>
 __device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, int lane, CrossSeq& s, int* faults = nullptr) {
-    int64_t kv = 0, q = 0, items = 0;
+    int64_t kv = 0, items = 0;
     for (int base = 0; base < p.f.batch; base += 32) {
-        int len = 0, qlen = 0, kt = 0, qt = 0;
+        int len = 0, qlen = 0, kt = 0, mine = 0;
         if (base + lane < p.f.batch) {
             bool bad_len, bad_q;
             len = cross_len(p, base + lane, bad_len);
             qlen = cross_qlen(p, base + lane, bad_q);
-            qt = (qlen * p.f.real_group + kCrossTile - 1) / kCrossTile;
             kt = qlen > 0 ? (len + kCrossTile - 1) / kCrossTile : 0;
+            mine = KIND == 0 ? kt : (qlen * p.f.real_group + KIND * kCrossTile - 1) / (KIND == 0 ? 1 : KIND * kCrossTile);
             if (faults) *faults += bad_len + bad_q;
         }
-        const int mine = KIND == 0 ? kt : (qt + KIND - 1) / (KIND == 0 ? 1 : KIND);
-        int kt_to = kt, qt_to = qt, to = mine;
+        int kt_to = kt, to = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, kt_to, o), c = __shfl_up_sync(0xffffffffu, qt_to, o), d = __shfl_up_sync(0xffffffffu, to, o);
-            if (lane >= o) { kt_to += a; qt_to += c; to += d; }
+            const int a = __shfl_up_sync(0xffffffffu, kt_to, o), c = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) { kt_to += a; to += c; }
         }
-        const bool kv_fits = kv + kt_to <= p.kv_room, q_fits = q + qt_to <= p.q_room;
-        if (faults) *faults += (kt > 0 && !kv_fits) + (qt > 0 && !q_fits);
+        const bool kv_fits = kv + kt_to <= p.kv_room;
+        if (faults) *faults += kt > 0 && !kv_fits;
         const uint32_t hit = __ballot_sync(0xffffffffu, index < items + to);
         if (hit) {
             const int l = __ffs(hit) - 1;
             s.b = base + l;
             s.local = (int)(index - items) - __shfl_sync(0xffffffffu, to - mine, l);
             s.len = __shfl_sync(0xffffffffu, kv_fits ? len : 0, l);
-            s.qlen = __shfl_sync(0xffffffffu, q_fits ? qlen : 0, l);
+            s.qlen = __shfl_sync(0xffffffffu, qlen, l);
             s.kv0 = (int)(kv + __shfl_sync(0xffffffffu, kt_to - kt, l));
-            s.q0 = (int)(q + __shfl_sync(0xffffffffu, qt_to - qt, l));
             return true;
         }
         kv += __shfl_sync(0xffffffffu, kt_to, 31);
-        q += __shfl_sync(0xffffffffu, qt_to, 31);
         items += __shfl_sync(0xffffffffu, to, 31);
     }
     return false;
@@ -159,6 +154,20 @@ __device__ __forceinline__ uint4 cross_turn(int dim, int c, bool negative) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// Piece c (eight dims, negative: a bit each) of row col of the matrix of the way in, which rotates the queries: column col of a query image is dim col ^ 1, as the codes have
+// them.  one: a pair of ones of the queries' type.
+__device__ __forceinline__ uint4 cross_way_in(int col, int c, uint32_t negative, uint32_t one) {
+    const int j = col ^ 1;
+    const uint32_t same = (uint32_t)__popc(j & (8 * c));
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t a = (same ^ (uint32_t)__popc(j & (2 * e)) ^ (negative >> (2 * e))) & 1u, b = (same ^ (uint32_t)__popc(j & (2 * e + 1)) ^ (negative >> (2 * e + 1))) & 1u;
+        v[e] = one | a << 15 | b << 31;
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // ---------------------------------------------------------------------------------------------
 // images laid out ahead
 // ---------------------------------------------------------------------------------------------
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
     __shared__ int64_t slot_s[kCrossTile];            // byte of each token's K slot
     __shared__ uint16_t norm_s[2][kCrossTile];
     __shared__ float most_s[2][4];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, H = p.f.kv_heads, G = p.f.real_group;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, H = p.f.kv_heads;
     grid_launch_dependents();
     for (int i = tid; i < 256 * 32; i += kLayThreads) lut[i] = (uint32_t)p.level_h[(i >> 5) & 15] | ((uint32_t)p.level_h[i >> 9] << 16);
     grid_dependency_wait();
@@ -186,7 +195,6 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
     }
     __syncthreads();
 
-    // ---- tiles of tokens -------------------------------------------------------------------------------
     const uint8_t* lut_lane = reinterpret_cast<const uint8_t*>(lut) + 4 * lane;
     auto level2 = [&](uint32_t byte) { return *reinterpret_cast<const uint32_t*>(lut_lane + (byte << 7)); };
     int64_t unit = blockIdx.x;
@@ -269,62 +277,6 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
             for (int d = 0; d < 8; d++) *reinterpret_cast<uint4*>(image + kCrossImage + cross_piece(16 * d + word, c)) = make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
         }
         __syncthreads();
-    }
-
-    // ---- tiles of query rows: a warp a row ------------------------------------------------------------
-    const float4 sign = reinterpret_cast<const float4*>(p.f.signs)[lane];
-    int64_t tiles = 0;                                // units are dealt on from where the tiles of tokens ended
-    {
-        int64_t kv = 0;
-        for (int base = 0; base < p.f.batch; base += 32) {
-            int kt = 0;
-            if (base + lane < p.f.batch) {
-                bool bad;
-                const int len = cross_len(p, base + lane, bad);
-                if (cross_qlen(p, base + lane, bad) > 0) kt = (len + kCrossTile - 1) / kCrossTile;
-            }
-            kv += __reduce_add_sync(0xffffffffu, kt);
-        }
-        tiles = kv * H;
-    }
-    for (unit -= tiles;; unit += gridDim.x) {
-        CrossSeq s;
-        const int64_t tile = unit / H;
-        const int h = (int)(unit - tile * H);
-        if (!cross_find<1>(p, tile, lane, s)) break;
-        if (s.qlen == 0) continue;
-        constexpr int kParts = EXACT ? 2 : 1;
-        uint8_t* const image = p.q_images + (tile * H + h) * kParts * kCrossImage;
-        const int row0 = s.local * kCrossTile, rows = s.qlen * G, first = p.cu_q[s.b];
-        for (int r = warp; r < kCrossTile; r += kLayThreads / 32) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const int row = row0 + r;
-            if (row < rows) {
-                const int qi = row / G, g = row - qi * G;
-                split_load_row<4>(p.f.q, p.f.q_dtype, (int64_t)(first + qi) * p.f.real_heads + h * G + g, p.f.head_dim, 4 * lane, v);
-            }
-            v[0] *= sign.x; v[1] *= sign.y; v[2] *= sign.z; v[3] *= sign.w;
-            split_fwht<4>(v, lane);
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[i] *= p.f.scale;
-                top = fmaxf(top, fabsf(v[i]));
-            }
-            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-            const int by = cross_exponent(top, 9);    // to [512, 1024)
-            const float f = p.f.k_scale < 0.0f ? -cross_power(by) : cross_power(by);
-            if (lane == 0) p.q_scales[(tile * H + h) * kCrossTile + r] = fabsf(p.f.k_scale) * cross_power(-by);
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] *= f;
-            const uint32_t at = cross_piece(r, lane >> 1) + 8 * (lane & 1);
-            const uint32_t a = pack_half2(v[1], v[0]), b = pack_half2(v[3], v[2]);
-            *reinterpret_cast<uint2*>(image + at) = make_uint2(a, b);
-            if constexpr (EXACT) {
-                const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-                *reinterpret_cast<uint2*>(image + kCrossImage + at) = make_uint2(pack_half2(v[1] - fa.x, v[0] - fa.y), pack_half2(v[3] - fb.x, v[2] - fb.y));
-            }
-        }
     }
 }
 
@@ -437,11 +389,11 @@ struct CrossMap {
     // Images in turn, of K and V.  Two tiles of query rows: K0 V0 K1 V1 ... ; one: K0 K1 V0 K2 V1 ... , the order in which they are needed.  Behind the last comes
     // the matrix of the way back, where the next K would be.  Looked up here each is written as two halves (64 tokens); it is free when its product has been formed.
     static constexpr int kImages = LAID ? 5 : 3;
-    static constexpr uint32_t kImg = kQ + 2 * kCrossImage;               // (before the first: the query rows as they come)
+    static constexpr uint32_t kImg = kQ + 2 * kCrossImage;
+    static constexpr uint32_t kWay = kImg + (kImages - 1) * kCrossImage; // before its first image: the matrix of the way in
     // The norms of tile t at t % 4: for the rows (exact), fp16, K's and V's; or for the look-ups, fp16, K's twice each.  When S (t - 2) has been formed P (t - 4)
     // has been handed over, so nobody reads the norms of tile t - 4 any more.
     static constexpr uint32_t kNorms = kImg + kImages * kCrossImage;
-    static constexpr uint32_t kQScale = kNorms;                          // (before the first norms)
     static constexpr int kNormBytes = EXACT ? 2 * kCrossTile * 2 : LAID ? 0 : 2 * kCrossTile * 4;
     static constexpr uint32_t kNormsEnd = kNorms + (kCrossMetas * kNormBytes > kCrossTile * 16 ? kCrossMetas * kNormBytes : kCrossTile * 16);      // (behind the last: sums of a group)
     static constexpr size_t kSmem = kNormsEnd - 1024;
@@ -464,6 +416,7 @@ template <bool EXACT, bool LAID>
 __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cross_attend_kernel(const __grid_constant__ CrossParams p) {
     constexpr int kTiles = EXACT ? 1 : 2;             // of query rows
     using M = CrossMap<EXACT, LAID>;
+    constexpr int kThreads = LAID ? kCrossRowThreads : kCrossThreads;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, H = p.f.kv_heads, G = p.f.real_group;
     uint8_t* const window = smem - smem_u32(smem);    // address 0 of the block's window
@@ -476,7 +429,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
     const uint32_t bars = M::kBars;
     const uint32_t raw_full = bars, raw_empty = raw_full + 16 * kCrossStages, meta_full = raw_empty + 16 * kCrossStages, s_formed = meta_full + 8 * kCrossMetas,
                    img_full = s_formed + 8 * kCrossMetas, img_empty = img_full + 16 * M::kImages, s_full = img_empty + 8 * M::kImages, p_full = s_full + 16,
-                   o_full = p_full + 16, a_full = o_full + 16, d_full = a_full + 16, drained = d_full + 16;      // raw: K's stages, then V's; images: two halves
+                   o_full = p_full + 16, a_full = o_full + 16, d_full = a_full + 16, drained = d_full + 16, turned = drained + 8;      // raw: K's stages, then V's; images: two halves
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(window + M::kBars + 400);
     volatile int* const gone = reinterpret_cast<volatile int*>(window + M::kBars + 404);
     if (tid == 9 * 32) {
@@ -501,6 +454,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             cross_bar_init(d_full + 8 * i, 1);
         }
         cross_bar_init(drained, 1);
+        cross_bar_init(turned, 1);
         *gone = 0;
         fence_barrier_init();
     }
@@ -528,7 +482,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
     CrossSeq s;
     const int64_t item = blockIdx.x / p.splits;
     const int split = (int)(blockIdx.x - item * p.splits), h = (int)(item % H);
-    if (!cross_find<kTiles>(p, item / H, lane, s) || s.qlen == 0) return; // uniform over the block
+    if (!cross_find<kTiles>(p, item / H, lane, s)) return;                // uniform over the block
     const int rows = s.qlen * G, row0 = s.local * kTiles * kCrossTile;
     const bool solo = kTiles == 1 || rows - row0 <= kCrossTile;           // one tile of query rows
     const int all = (s.len + kCrossTile - 1) / kCrossTile;
@@ -564,92 +518,46 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         if (lane < some)
             split_box(kCrossRaw + (ring8 + stage) * kCrossUnit + lane * kPageTokens * kSlotBytes, &p.f.cache_map, h * kSlotBytes, id * kPageTokens, which, bar);
     };
-    if constexpr (!LAID) {
-        // Query rows, as they come, into shared memory: 16-bit rows of whole pieces of 16 bytes by asynchronous copies, all in flight together.
-        const int q_rows = min(rows - row0, solo ? kCrossTile : 2 * kCrossTile), q_first = p.cu_q[s.b];
-        const bool plain = p.f.q_dtype != TQ_F32 && D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f.q) & 15) == 0;
-        auto row_of = [&](int r) -> int64_t {             // of the query tensor
-            const int row = row0 + r, qi = row / G;
-            return (int64_t)(q_first + qi) * p.f.real_heads + h * G + (row - qi * G);
-        };
-        if (plain) {
-            const int pieces = D / 8;
-            for (int i = tid; i < q_rows * pieces; i += kCrossThreads) {
-                const int r = i / pieces, c = i - r * pieces;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(M::kImg + r * 256 + 16 * c), "l"(reinterpret_cast<const uint16_t*>(p.f.q) + row_of(r) * D + 8 * c) : "memory");
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-        }
-        __syncthreads();
-        if (warp == 8 || warp == 11) {
-            id_now = page_id(lane);
-            id_next = page_id(32 + lane);
-            for (int u = 0; u < min(units, kCrossStages); u++) copy_unit(u);
-        }
-        // Rotated, by a power of two to [512, 1024), into the images.  Sixteen warps take rows warp, warp + 16, ... , two at a time.
-        if (warp < 8 || warp >= 12) {
-            const float4 sign = reinterpret_cast<const float4*>(p.f.signs)[lane];
+    // The queries: 16-bit rows as they come into the images' place (asynchronous copies, all in flight together), and the matrix that rotates them.
+    const int q_tiles = solo ? 1 : 2, q_rows = min(rows - row0, q_tiles * kCrossTile), q_first = p.cu_q[s.b];
+    const bool halves = p.f.q_dtype != TQ_F32;
+    auto row_of = [&](int r) -> int64_t {             // of the query tensor
+        const int row = row0 + r, qi = row / G;
+        return (int64_t)(q_first + qi) * p.f.real_heads + h * G + (row - qi * G);
+    };
+    if (halves && n > 0) {
+        const uint16_t* const q16 = reinterpret_cast<const uint16_t*>(p.f.q);
+        const bool whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(q16) & 15) == 0;
 #pragma unroll 1
-            for (int r0 = warp < 8 ? warp : warp - 4; r0 < (solo ? kCrossTile : 2 * kCrossTile); r0 += 2 * 16) {
-                float v[2][4], top[2];
+        for (int i = tid; i < q_tiles * kCrossTile * 16; i += kThreads) {
+            const int r = i >> 4, c = i & 15, some = r < q_rows ? min(8, D - 8 * c) : 0;
+            const uint32_t to = M::kQ + (r >> 7) * kCrossImage + cross_piece(r & 127, c);
+            const uint16_t* const from = some > 0 ? q16 + row_of(r) * D + 8 * c : q16;
+            if (whole) {                              // (no bytes: zeros)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(some > 0 ? 16 : 0) : "memory");
+            } else {
+                uint32_t v[4];
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int r = r0 + 16 * u;
-                    const bool in = r < q_rows && 4 * lane < D;
-                    if (!plain) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) v[u][i] = in && 4 * lane + i < D ? load_q(p.f.q, p.f.q_dtype, row_of(r) * D + 4 * lane + i) : 0.0f;
-                    } else {
-                        const uint2 raw = in ? lds64(M::kImg + r * 256 + 8 * lane) : make_uint2(0u, 0u);
-                        if (p.f.q_dtype == TQ_BF16) {
-                            v[u][0] = __uint_as_float(raw.x << 16); v[u][1] = __uint_as_float(raw.x & 0xffff0000u);
-                            v[u][2] = __uint_as_float(raw.y << 16); v[u][3] = __uint_as_float(raw.y & 0xffff0000u);
-                        } else {
-                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
-                            v[u][0] = a.x; v[u][1] = a.y; v[u][2] = b.x; v[u][3] = b.y;
-                        }
-                    }
-                    v[u][0] *= sign.x; v[u][1] *= sign.y; v[u][2] *= sign.z; v[u][3] *= sign.w;
-                    split_fwht<4>(v[u], lane);
-                    top[u] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        v[u][i] *= p.f.scale;
-                        top[u] = fmaxf(top[u], fabsf(v[u][i]));
-                    }
-                    top[u] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top[u])));
-                }
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int r = r0 + 16 * u, by = cross_exponent(top[u], 9);
-                    const float f = p.f.k_scale < 0.0f ? -cross_power(by) : cross_power(by);
-                    if (lane == 0) reinterpret_cast<float*>(window + M::kQScale)[r] = fabsf(p.f.k_scale) * cross_power(-by);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[u][i] *= f;
-                    uint8_t* const to = window + M::kQ + (r >> 7) * kCrossImage + cross_piece(r & 127, lane >> 1) + 8 * (lane & 1);
-                    const uint32_t a = pack_half2(v[u][1], v[u][0]), b = pack_half2(v[u][3], v[u][2]);      // pairs {odd, even}, as the codes have them
-                    *reinterpret_cast<uint2*>(to) = make_uint2(a, b);
-                    if constexpr (EXACT) {
-                        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-                        *reinterpret_cast<uint2*>(to + kCrossImage) = make_uint2(pack_half2(v[u][1] - fa.x, v[u][0] - fa.y), pack_half2(v[u][3] - fb.x, v[u][2] - fb.y));
-                    }
-                }
+                for (int e = 0; e < 4; e++) v[e] = (2 * e < some ? (uint32_t)from[2 * e] : 0u) | (2 * e + 1 < some ? (uint32_t)from[2 * e + 1] << 16 : 0u);
+                cross_sts(to, v[0], v[1], v[2], v[3]);
             }
-            fence_proxy_async();
         }
+        const uint32_t one = p.f.q_dtype == TQ_BF16 ? 0x3F803F80u : 0x3C003C00u;
+        uint32_t negative = 0;                        // a thread's pieces are all of the same eight dims
+#pragma unroll
+        for (int e = 0; e < 8; e++) negative |= (uint32_t)(p.f.signs[8 * (tid & 15) + e] < 0.0f) << e;
+#pragma unroll 1
+        for (int i = tid; i < kCrossTile * 16; i += kThreads) {
+            const uint4 v = cross_way_in(i >> 4, i & 15, negative, one);
+            cross_sts(M::kWay + cross_piece(i >> 4, i & 15), v.x, v.y, v.z, v.w);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;                 // S / P of group i at 128 i, O at 256 + 128 i; all 512 columns: zero
-    const int64_t q_unit = (int64_t)(s.q0 + s.local * kTiles) * H + h;                    // the block's query images: this, and H on
-    float q_scale = 0.0f;
-    if constexpr (LAID) {
-        if (warp < 8) q_scale = p.q_scales[(q_unit + (solo ? 0 : (warp >> 2) * H)) * kCrossTile + (tid & 127)];
-    } else {
-        if (warp < 8) q_scale = reinterpret_cast<const float*>(window + M::kQScale)[(solo ? 0 : (warp >> 2) * kCrossTile) + (tid & 127)];
-        __syncthreads();                              // the scales' place is the norms' from here on
-    }
 
     if (!LAID && warp >= 12) {
         const uint32_t lut_lane = kCrossLut + 4 * lane;
@@ -667,7 +575,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             ok = cross_wait(raw_full + 8 * (ring + stage), turn, gone);
             if (!EXACT && half == 0) ok = ok && cross_wait(meta_full + 8 * (t % kCrossMetas), (t / kCrossMetas) & 1, gone);
             const int item = on_k ? k_item(t) : v_item(t), slot = item % M::kImages;
-            if (half == 0) ok = ok && cross_wait(img_empty + 8 * slot, ((item / M::kImages) & 1) ^ 1, gone);
+            if (half == 0) ok = ok && cross_wait(img_empty + 8 * slot, ((item / M::kImages) & 1) ^ 1, gone) && (item != M::kImages - 1 || cross_wait(turned, 0, gone));
             if (!ok) break;
             const uint32_t image = M::kImg + slot * kCrossImage;
             if (on_k) {
@@ -756,7 +664,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         if (on_k && ok && n > 0 && p.splits == 1) {
             // =============================== the matrix of the way back ======================================
             const int item = k_item(n), slot = item % M::kImages;
-            ok = cross_wait(img_empty + 8 * slot, ((item / M::kImages) & 1) ^ 1, gone);
+            ok = cross_wait(img_empty + 8 * slot, ((item / M::kImages) & 1) ^ 1, gone) && (item != M::kImages - 1 || cross_wait(turned, 0, gone));
             if (ok) {
 #pragma unroll 1
                 for (int i = tid - 12 * 32; i < kCrossTile * 16; i += kCrossTeam * 32) {
@@ -772,19 +680,13 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (LAID && warp == 8) {
-            // =============================== copies: queries, images ======================================
-            constexpr int kParts = EXACT ? 2 : 1;
+            // =============================== copies: images ===============================================
             const int items = n == 0 ? 0 : solo || p.splits == 1 ? 2 * n + 1 : 2 * n;
             int k = 0;
-            if (lane == 0 && n > 0) {
-                const int q_images = solo ? kParts : 2;
-                split_expect(raw_full, (uint32_t)(q_images * kCrossImage));
-                for (int a = 0; a < q_images; a++) cross_copy(M::kQ + a * kCrossImage, p.q_images + ((q_unit + (EXACT ? 0 : a) * H) * kParts + (EXACT ? a : 0)) * kCrossImage, kCrossImage, raw_full);
-            }
             for (; k < items; k++) {
                 const int slot = k % M::kImages, v = solo ? k > 0 && !(k & 1) : k & 1, t = solo ? v ? (k >> 1) - 1 : (k + 1) >> 1 : k >> 1;      // item k is V (t) or K (t)
                 if (t == n && p.splits > 1) continue;
-                if (!cross_wait(img_empty + 8 * slot, ((k / M::kImages) & 1) ^ 1, gone)) break;
+                if (!cross_wait(img_empty + 8 * slot, ((k / M::kImages) & 1) ^ 1, gone) || (k == M::kImages - 1 && !cross_wait(turned, 0, gone))) break;
                 if (lane == 0) {
                     const uint8_t* const from = t == n ? p.turn_image : p.kv_images + (((int64_t)(s.kv0 + j0 + t) * H + h) * 2 + v) * kCrossImage;
                     split_expect(img_full + 16 * slot + 8, kCrossImage);
@@ -795,8 +697,6 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             if (k < items) {                          // gave up: what is in flight gets its time to land
                 if (lane == 0) atomicAdd(&g_cross_faults, 1);
                 *gone = 1;
-                for (uint32_t w = 0; w < kCrossWaitLimit / 64; w++)
-                    if (split_try_wait(raw_full, 0)) break;
                 for (int c = k > M::kImages ? k - M::kImages : 0; c < k; c++)
                     for (uint32_t w = 0; w < kCrossWaitLimit / 64; w++)
                         if (split_try_wait(img_full + 16 * (c % M::kImages) + 8, (c / M::kImages) & 1)) break;
@@ -826,9 +726,11 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             if (!ok) *gone = 1;
         } else if (!LAID && (warp == 8 || warp == 11)) {
             // =============================== copies: K, V ================================================
-            int u = min(units, kCrossStages);
+            id_now = page_id(lane);
+            id_next = page_id(32 + lane);
+            int u = 0;
             for (; u < units; u++) {
-                if ((u & 7) == 0) {
+                if ((u & 7) == 0 && u > 0) {
                     id_now = id_next;
                     id_next = page_id(4 * u + 32 + lane);
                 }
@@ -925,7 +827,22 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 for (int kk = 0; kk < 4; kk++) mq_mma_ts(256 + 128 * i, 128 * i + 32 * half + 8 * kk, v_desc + (uint64_t)(kk * 2), idesc, more || half || kk ? 1u : 0u);
             };
             auto image_there = [&](int item, int half) { return cross_wait(img_full + 16 * (item % M::kImages) + (LAID ? 8 : 8 * half), (item / M::kImages) & 1, gone); };
-            bool ok = !LAID || cross_wait(raw_full, 0, gone);      // the queries
+            bool ok = true;
+            if (halves && elect_one()) {              // the queries' rotation: their own type against ones, into S's place
+                const uint32_t q_idesc = idesc | (p.f.q_dtype == TQ_BF16 ? 1u << 7 | 1u << 10 : 0u);
+                const uint64_t way = cross_desc(M::kWay);
+#pragma unroll 1
+                for (int kk = 0; kk < 8 * q_tiles; kk++) {
+                    const uint64_t off = (uint64_t)(((kk >> 2) & 1) * 1024 + (kk & 3) * 2);
+                    mq_mma(128 * (kk >> 3), q_desc + (uint64_t)(kk >> 3) * kImage16 + off, way + off, q_idesc, kk & 7 ? 1u : 0u);
+                }
+                cross_commit(turned);
+            }
+            __syncwarp();
+            asm volatile("bar.sync 2, 288;" ::: "memory");         // the rows' warps have written the images
+            tc_fence_after();
+            if (!halves && elect_one()) cross_commit(turned);
+            __syncwarp();
             // Two tiles of query rows: step u is group u % 2 and tile u / 2 of the tokens; one: group u % 2, tile u.  After P V of a step comes the next S
             // of its group.
             const int first = solo ? min(2, n) : 1, steps = solo ? n : 2 * n;
@@ -1017,6 +934,77 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tm_s = tmem + 128 * i + lane_at, tm_o = tmem + 256 + 128 * i + lane_at;
         bool ok = true;
+        // ---- the queries: rotated, by a power of two to [512, 1024), into the images.  One tile: half of a row's columns each group --------------
+        float q_scale = 0.0f;
+        if (n > 0) {
+            const uint32_t image = M::kQ + (solo ? 0 : i) * kCrossImage;
+            auto take = [&](float top) {              // the largest of the row: what its numbers are multiplied by
+                const int by = cross_exponent(top * p.f.scale, 9);
+                q_scale = fabsf(p.f.k_scale) * cross_power(-by);
+                return (p.f.k_scale < 0.0f ? -cross_power(by) : cross_power(by)) * p.f.scale;
+            };
+            if (halves) {
+                ok = cross_wait(turned, 0, gone);
+                tc_fence_after();
+                if (ok) {
+                    float top = 0.0f, v[32];
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        cross_ld(tm_s - (solo ? 128 * i : 0) + 32 * c, v);
+                        cross_ld_wait(v);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) top = fmaxf(top, fabsf(v[e]));
+                    }
+                    const float f = take(top);
+#pragma unroll 1
+                    for (int c = solo ? 2 * i : 0; c < (solo ? 2 * i + 2 : 4); c++) {
+                        cross_ld(tm_s - (solo ? 128 * i : 0) + 32 * c, v);
+                        cross_ld_wait(v);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t a[4], b[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const float x = v[8 * e + 2 * k] * f, y = v[8 * e + 2 * k + 1] * f;
+                                a[k] = pack_half2(x, y);
+                                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&a[k]));
+                                b[k] = pack_half2(x - back.x, y - back.y);
+                            }
+                            cross_sts(image + cross_piece(r, 4 * c + e), a[0], a[1], a[2], a[3]);
+                            if constexpr (EXACT) cross_sts(image + kCrossImage + cross_piece(r, 4 * c + e), b[0], b[1], b[2], b[3]);
+                        }
+                    }
+                }
+            } else {                                  // 32-bit queries: a warp a row, each warp the rows of its threads
+                const float4 sign = reinterpret_cast<const float4*>(p.f.signs)[lane];
+#pragma unroll 1
+                for (int j = 0; j < 32; j++) {
+                    const int rr = (warp & 3) * 32 + j, rq = rr + (solo ? 0 : i * kCrossTile);
+                    float v[4], top = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = rq < q_rows && 4 * lane + e < D ? load_q(p.f.q, TQ_F32, row_of(rq) * D + 4 * lane + e) : 0.0f;
+                    v[0] *= sign.x; v[1] *= sign.y; v[2] *= sign.z; v[3] *= sign.w;
+                    split_fwht<4>(v, lane);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(v[e]));
+                    const float keep = q_scale, f = take(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+                    if (lane != j) q_scale = keep;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] *= f;
+                    if (solo && i == 1) continue;     // (the first group writes them)
+                    const uint32_t a = pack_half2(v[1], v[0]), b = pack_half2(v[3], v[2]), to = image + cross_piece(rr, lane >> 1) + 8 * (lane & 1);
+                    *reinterpret_cast<uint2*>(window + to) = make_uint2(a, b);
+                    if constexpr (EXACT) {
+                        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
+                        *reinterpret_cast<uint2*>(window + to + kCrossImage) = make_uint2(pack_half2(v[1] - fa.x, v[0] - fa.y), pack_half2(v[3] - fb.x, v[2] - fb.y));
+                    }
+                }
+            }
+            fence_proxy_async();
+            tc_fence_before();
+            asm volatile("bar.sync 2, 288;" ::: "memory");
+            if (!ok) *gone = 1;
+        }
         float m = kNoMax, l = 0.0f, ev_ref = kCrossNoNorm;
         const int turns = solo ? (n + 1 - i) >> 1 : n;
         for (int k = 0; k < turns && ok; k++) {
@@ -1353,9 +1341,9 @@ static size_t cross_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct CrossLayout {
     bool laid;
-    int64_t items, kv_room, q_room;     // tiles or pairs of tiles of query rows, tiles of tokens and of query rows, at most
+    int64_t items, kv_room;     // tiles or pairs of tiles of query rows, tiles of tokens, at most
     int splits;
-    size_t turn, scales, norms, q_images, q_scales, partial_lse, partial_o, end;      // the images of K and V are in front
+    size_t turn, scales, norms, partial_lse, partial_o, end;      // the images of K and V are in front
 };
 static bool cross_exact(int out_dtype) { return out_dtype != TQ_BF16; }
 static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, int heads, int kv_heads, int max_pages, int out_dtype, int sms) {
@@ -1364,7 +1352,6 @@ static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, in
     const int64_t per = (exact ? 1 : 2) * kCrossTile, rows = (int64_t)total_q * (heads / kv_heads);
     l.items = rows / per + batch;                           // every sequence may end inside one
     l.kv_room = total_tokens / kCrossTile + batch;
-    l.q_room = rows / kCrossTile + batch;
     l.laid = rows > kCrossLaid * per * batch;
     // As many cuts of the tokens as fill the SMs, of two tiles (one a warpgroup) at least.
     const int64_t some = (rows + per - 1) / per, blocks = (some > batch ? some : batch) * kv_heads;
@@ -1372,13 +1359,11 @@ static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, in
     const int64_t most = (longest + 2 * kCrossTile - 1) / (2 * kCrossTile), fit = sms / blocks;
     l.splits = (int)(fit < most ? fit : most);
     if (l.splits < 1) l.splits = 1;
-    const size_t units = l.laid ? (size_t)l.kv_room * kv_heads : 0, q_units = l.laid ? (size_t)l.q_room * kv_heads : 0, parts = exact ? 2 : 1;
+    const size_t units = l.laid ? (size_t)l.kv_room * kv_heads : 0;
     l.turn = units * 2 * kCrossImage;
     l.scales = l.turn + (l.laid ? kCrossImage : 0);
     l.norms = l.scales + cross_up(units * sizeof(float2));
-    l.q_images = l.norms + (exact ? cross_up(units * 2 * kCrossTile * 2) : 0);
-    l.q_scales = l.q_images + q_units * parts * kCrossImage;
-    l.partial_lse = l.q_scales + cross_up(q_units * kCrossTile * 4);
+    l.partial_lse = l.norms + (exact ? cross_up(units * 2 * kCrossTile * 2) : 0);
     const size_t cut = l.splits > 1 ? (size_t)l.splits * total_q * heads : 0;
     l.partial_o = l.partial_lse + cross_up(cut * 4);
     l.end = l.partial_o + cross_up(cut * kCrossTile * 4);
@@ -1396,7 +1381,7 @@ static int launch_cross(const CrossParams& p, int sms, int64_t blocks, cudaStrea
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     if constexpr (LAID) {
-        const int64_t units = (p.kv_room + p.q_room) * p.f.kv_heads, lay = units < 4 * sms ? units : 4 * sms;
+        const int64_t units = p.kv_room * p.f.kv_heads, lay = units < 4 * sms ? units : 4 * sms;
         TQ_CUDA(launch_serialized(cross_lay_out_kernel<EXACT>, dim3((unsigned)lay), dim3(kLayThreads), 0, s, p));
     }
     TQ_CUDA(launch_serialized(cross_attend_kernel<EXACT, LAID>, dim3((unsigned)blocks), dim3(LAID ? kCrossRowThreads : kCrossThreads), kSmem, s, p));
@@ -1466,11 +1451,8 @@ extern "C" int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* 
     p.turn_image = ws + l.turn;
     p.tile_scales = reinterpret_cast<float2*>(ws + l.scales);
     p.tile_norms = reinterpret_cast<uint16_t*>(ws + l.norms);
-    p.q_images = ws + l.q_images;
-    p.q_scales = reinterpret_cast<float*>(ws + l.q_scales);
     p.partial_lse = reinterpret_cast<float*>(ws + l.partial_lse);
     p.kv_room = l.kv_room;
-    p.q_room = l.q_room;
     p.partial_o = reinterpret_cast<float*>(ws + l.partial_o);
     p.total_q = total_q;
     p.splits = l.splits;
