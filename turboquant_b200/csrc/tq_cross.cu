@@ -55,7 +55,7 @@ struct CrossParams {
     const int32_t* cu_q;        // [batch + 1]
     // where the images are laid out ahead:
     uint8_t* kv_images;         // [tile][head][K, V][32 KB]; behind the last, the matrix of the way back
-    uint8_t* turn_image;
+    uint8_t* turn_image;        // and the matrix of the way in behind it
     float2* tile_scales;        // [tile][head]: K's power of two, the logarithm of V's
     uint16_t* tile_norms;       // exact: [tile][head][K, V][128]
     int64_t kv_room;            // tiles that there is room for
@@ -154,6 +154,12 @@ __device__ __forceinline__ uint4 cross_turn(int dim, int c, bool negative) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+__device__ __forceinline__ uint32_t cross_negative(const float* signs, int c) {      // of eight dims, a bit each
+    uint32_t negative = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) negative |= (uint32_t)(signs[8 * c + e] < 0.0f) << e;
+    return negative;
+}
 // Piece c (eight dims, negative: a bit each) of row col of the matrix of the way in, which rotates the queries: column col of a query image is dim col ^ 1, as the codes have
 // them.  one: a pair of ones of the queries' type.
 __device__ __forceinline__ uint4 cross_way_in(int col, int c, uint32_t negative, uint32_t one) {
@@ -189,9 +195,12 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
         cross_find<0>(p, (int64_t)1 << 60, lane, s, &faults);
         if (faults) atomicAdd(&g_cross_faults, faults);
     }
-    if (blockIdx.x == gridDim.x - 1) {                // the matrix of the way back
-        for (int i = tid; i < kCrossTile * 16; i += kLayThreads)
+    if (blockIdx.x == gridDim.x - 1) {                // the matrices of the way back and in
+        const uint32_t one = p.f.q_dtype == TQ_BF16 ? 0x3F803F80u : 0x3C003C00u, negative = cross_negative(p.f.signs, tid & 15);
+        for (int i = tid; i < kCrossTile * 16; i += kLayThreads) {
             *reinterpret_cast<uint4*>(p.turn_image + cross_piece(i >> 4, i & 15)) = cross_turn(i >> 4, i & 15, p.f.signs[i >> 4] < 0.0f);
+            *reinterpret_cast<uint4*>(p.turn_image + kCrossImage + cross_piece(i >> 4, i & 15)) = cross_way_in(i >> 4, i & 15, negative, one);
+        }
     }
     __syncthreads();
 
@@ -487,6 +496,10 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
     const bool solo = kTiles == 1 || rows - row0 <= kCrossTile;           // one tile of query rows
     const int all = (s.len + kCrossTile - 1) / kCrossTile;
     const int j0 = (int)((int64_t)all * split / p.splits), n = (int)((int64_t)all * (split + 1) / p.splits) - j0;      // the block's tiles of tokens
+    if (LAID && tid == 9 * 32 && n > 0) {             // the matrix of the way in, see below
+        split_expect(raw_full, kCrossImage);
+        cross_copy(M::kWay, p.turn_image + kCrossImage, kCrossImage, raw_full);
+    }
 
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(M::kBars + 400), "r"(512));
@@ -528,11 +541,20 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
     if (halves && n > 0) {
         const uint16_t* const q16 = reinterpret_cast<const uint16_t*>(p.f.q);
         const bool whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(q16) & 15) == 0;
+        constexpr int kStep = kThreads / 16;          // rows on: a query row's place moves by on_q queries and on_g heads
+        const int c = tid & 15, on_q = kStep / G, on_g = kStep - on_q * G;
+        int r = tid >> 4, qi = (row0 + r) / G, g = row0 + r - qi * G;
 #pragma unroll 1
-        for (int i = tid; i < q_tiles * kCrossTile * 16; i += kThreads) {
-            const int r = i >> 4, c = i & 15, some = r < q_rows ? min(8, D - 8 * c) : 0;
+        for (; r < q_tiles * kCrossTile; r += kStep) {
+            const int some = r < q_rows ? min(8, D - 8 * c) : 0;
             const uint32_t to = M::kQ + (r >> 7) * kCrossImage + cross_piece(r & 127, c);
-            const uint16_t* const from = some > 0 ? q16 + row_of(r) * D + 8 * c : q16;
+            const uint16_t* const from = some > 0 ? q16 + ((int64_t)(q_first + qi) * p.f.real_heads + h * G + g) * D + 8 * c : q16;
+            qi += on_q;
+            g += on_g;
+            if (g >= G) {
+                g -= G;
+                qi++;
+            }
             if (whole) {                              // (no bytes: zeros)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(some > 0 ? 16 : 0) : "memory");
             } else {
@@ -542,14 +564,14 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 cross_sts(to, v[0], v[1], v[2], v[3]);
             }
         }
-        const uint32_t one = p.f.q_dtype == TQ_BF16 ? 0x3F803F80u : 0x3C003C00u;
-        uint32_t negative = 0;                        // a thread's pieces are all of the same eight dims
-#pragma unroll
-        for (int e = 0; e < 8; e++) negative |= (uint32_t)(p.f.signs[8 * (tid & 15) + e] < 0.0f) << e;
+        if constexpr (!LAID) {
+            const uint32_t one = p.f.q_dtype == TQ_BF16 ? 0x3F803F80u : 0x3C003C00u;
+            const uint32_t negative = cross_negative(p.f.signs, c);
 #pragma unroll 1
-        for (int i = tid; i < kCrossTile * 16; i += kThreads) {
-            const uint4 v = cross_way_in(i >> 4, i & 15, negative, one);
-            cross_sts(M::kWay + cross_piece(i >> 4, i & 15), v.x, v.y, v.z, v.w);
+            for (int col = tid >> 4; col < kCrossTile; col += kStep) {
+                const uint4 v = cross_way_in(col, c, negative, one);
+                cross_sts(M::kWay + cross_piece(col, c), v.x, v.y, v.z, v.w);
+            }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
@@ -827,8 +849,8 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 for (int kk = 0; kk < 4; kk++) mq_mma_ts(256 + 128 * i, 128 * i + 32 * half + 8 * kk, v_desc + (uint64_t)(kk * 2), idesc, more || half || kk ? 1u : 0u);
             };
             auto image_there = [&](int item, int half) { return cross_wait(img_full + 16 * (item % M::kImages) + (LAID ? 8 : 8 * half), (item / M::kImages) & 1, gone); };
-            bool ok = true;
-            if (halves && elect_one()) {              // the queries' rotation: their own type against ones, into S's place
+            bool ok = !LAID || cross_wait(raw_full, 0, gone);
+            if (ok && halves && elect_one()) {              // the queries' rotation: their own type against ones, into S's place
                 const uint32_t q_idesc = idesc | (p.f.q_dtype == TQ_BF16 ? 1u << 7 | 1u << 10 : 0u);
                 const uint64_t way = cross_desc(M::kWay);
 #pragma unroll 1
@@ -1184,7 +1206,23 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             scale *= inv;
             scale_other *= inv;
             const int qi = row / G, g = row - qi * G;
-            const int64_t to = live ? (int64_t)(p.cu_q[s.b] + qi) * p.f.real_heads + h * G + g : 0, at = (int64_t)split * p.total_q * p.f.real_heads + to;
+            const int64_t to = live ? (int64_t)(q_first + qi) * p.f.real_heads + h * G + g : -1, at = (int64_t)split * p.total_q * p.f.real_heads + to;
+            // 64 bytes each of the warp's rows go to memory by way of shared memory (the queries' place), neighbouring lanes to neighbouring pieces of a row.
+            const uint32_t stage = M::kQ + i * kCrossImage + (warp & 3) * 2048;
+            auto place = [&](int row, int piece) { return stage + row * 64 + 16 * (piece ^ ((row >> 1) & 3)); };
+            auto rows_out = [&](const uint32_t* v, int at_byte) {
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 4; e++) cross_sts(place(lane, e), v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int r = 8 * j + (lane >> 2), piece = lane & 3;
+                    const uint4 x = lds128(place(r, piece));
+                    const int64_t row_to = __shfl_sync(0xffffffffu, to, r);
+                    if (row_to >= 0 && at_byte + 16 * piece < 2 * D) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.f.out) + row_to * 2 * D + at_byte + 16 * piece) = x;
+                }
+            };
             // The weighted mean, columns as O has them: a partial, or two fp16 parts in S's place for the way back (at most 2^15: a mean of rows of levels below 4 times
             // norms below 2^7, under powers of two up to 2^6).
 #pragma unroll 1
@@ -1253,24 +1291,19 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e++) v[e] = none ? 0.0f : v[e] * f;
-                    if (!live) continue;
                     if (whole) {
-                        uint16_t* const dst = reinterpret_cast<uint16_t*>(p.f.out) + to * D + 32 * c;
+                        uint32_t u[16];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            uint32_t u[4];
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                if (p.f.out_dtype == TQ_BF16) {
-                                    const __nv_bfloat162 t = __floats2bfloat162_rn(v[8 * e + 2 * k], v[8 * e + 2 * k + 1]);
-                                    u[k] = *reinterpret_cast<const uint32_t*>(&t);
-                                } else {
-                                    u[k] = pack_half2(v[8 * e + 2 * k], v[8 * e + 2 * k + 1]);
-                                }
+                        for (int e = 0; e < 16; e++) {
+                            if (p.f.out_dtype == TQ_BF16) {
+                                const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                                u[e] = *reinterpret_cast<const uint32_t*>(&t);
+                            } else {
+                                u[e] = pack_half2(v[2 * e], v[2 * e + 1]);
                             }
-                            if (32 * c + 8 * e < D) *reinterpret_cast<uint4*>(dst + 8 * e) = make_uint4(u[0], u[1], u[2], u[3]);
                         }
-                    } else {
+                        rows_out(u, 64 * c);
+                    } else if (live) {
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
                             if (32 * c + e >= D) continue;
@@ -1361,7 +1394,7 @@ static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, in
     if (l.splits < 1) l.splits = 1;
     const size_t units = l.laid ? (size_t)l.kv_room * kv_heads : 0;
     l.turn = units * 2 * kCrossImage;
-    l.scales = l.turn + (l.laid ? kCrossImage : 0);
+    l.scales = l.turn + (l.laid ? 2 * kCrossImage : 0);
     l.norms = l.scales + cross_up(units * sizeof(float2));
     l.partial_lse = l.norms + (exact ? cross_up(units * 2 * kCrossTile * 2) : 0);
     const size_t cut = l.splits > 1 ? (size_t)l.splits * total_q * heads : 0;
