@@ -20,7 +20,9 @@
 
 namespace tq {
 
-constexpr int kEvictThreads = 512;             // of a block of the selection, two an SM
+// Threads of a block of the selection: two blocks an SM; or one, where its share has no room in shared memory and each walk over it waits for L2 (a million tokens, 8 heads:
+// 138 us with 512 threads a block, 124 with 1024; shares of 16384 tokens in shared memory: 66.5 and 66.9).
+constexpr int kEvictThreads = 512, kEvictManyThreads = 1024;
 constexpr int kEvictRun = 128;                 // tokens of a warp's load: four a lane
 constexpr int kEvictAhead = 4;                 // loads in flight together
 constexpr int kEvictMaxCluster = 16;
@@ -104,8 +106,8 @@ __device__ __forceinline__ int cluster_load(const int* local, uint32_t rank) {
 }
 
 template <bool KEPT>
-__global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const __grid_constant__ EvictParams p) {
-    constexpr int THREADS = kEvictThreads, kWarps = THREADS / 32, kList = kEvictListBytes / 4 / kWarps;
+__global__ void __launch_bounds__(KEPT ? kEvictThreads : kEvictManyThreads, KEPT ? 2 : 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
+    constexpr int THREADS = KEPT ? kEvictThreads : kEvictManyThreads, kWarps = THREADS / 32, kList = kEvictListBytes / 4 / kWarps;
     extern __shared__ __align__(16) uint32_t evict_smem[];
     uint32_t* const hist = evict_smem;                            // [bin][column], then [digit][lane]
     uint32_t* const lists = evict_smem + kEvictDigitBytes / 4;
@@ -524,7 +526,7 @@ static int launch_select(EvictParams& p, int units, int C, int too_long, cudaStr
     TQ_CUDA(cudaGetDevice(&dev));
     TQ_REQUIRE(dev >= 0 && dev < 64, TQ_ERR_UNSUPPORTED, "device %d", dev);
     const auto kernel = evict_select_kernel<KEPT>;
-    constexpr int THREADS = kEvictThreads, kMost = kEvictHistBytes + (KEPT ? kEvictMostKeys * 4 : 0);
+    constexpr int THREADS = KEPT ? kEvictThreads : kEvictManyThreads, kMost = kEvictHistBytes + (KEPT ? kEvictMostKeys * 4 : 0);
     if (active[dev][1] == 0) {
         TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
         TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
