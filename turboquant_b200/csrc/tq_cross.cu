@@ -13,18 +13,24 @@
 //   a warp        issues S = Q K^^T and O += P V^,
 //   two warpgroups, a thread a row, take S from tensor memory, keep a running maximum and sum, and put P (fp16) into the same columns.
 //
-// Where many query rows share a sequence's tokens (prompts), a first kernel writes the images of K, V and the queries to memory once and a block only copies
-// them in, 32 KB each: the look-ups of four warps a team take longer than the products they feed (845 us looked up, 645 laid out ahead, at four sequences of 2048
-// queries on 4096 tokens, 32 heads on 8).  With few rows that would write and read 512 bytes for every 80-byte slot, and the slots are looked up as they come
-// (404 us laid out ahead, 177 looked up, at two sequences of 16 queries on 65536 tokens, 64 heads on 8).
+// Where many query rows share a sequence's tokens (prompts), a first kernel writes the images of K and V to memory once and a block only copies them in,
+// 32 KB each: the look-ups take longer than the products they feed (453 us looked up, 299 laid out ahead, at four sequences of 1024 queries on 4096
+// tokens, 32 heads on 8).  With few rows that would write and read 512 bytes for every 80-byte slot, and the slots are looked up as they
+// come (43 us looked up, 53 laid out ahead, with 32 queries).
 //
 // S, then P, and O of two tiles are all of tensor memory: 2 x (128 + 128) columns.  With two tiles of query rows each warpgroup has one, and while it works out
-// exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn, and the
-// first joins the second's sums to its own at the end.  The running maximum is raised only when a logit exceeds it by 2^8, which makes
-// rescaling O rare; a row needs no other thread but its own.  At the end O, as two fp16 parts, goes through the tensor core once more, against the Hadamard matrix
-// and the signs (exact in fp16), which brings its rows back from the rotation and its columns into order.  The code that runs once a block is kept short:
-// straight through 64 values in registers, fetched anew by every block, the butterflies took as long as ten tiles.  Where few rows have long sequences the tokens are cut over several blocks as well, whose
-// rows a second kernel joins.
+// exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn, and the first joins the second's
+// sums to its own at the end.  The running maximum is raised only when a logit exceeds it by 2^8, which makes rescaling O rare; a row needs no other
+// thread but its own.  Where few rows have long sequences the tokens are cut over several blocks as well, whose rows a second kernel joins.
+//
+// The rotations are matrix products too, with a matrix of ones and minus ones, exact in any type: the queries go through the tensor core as they come before the
+// first tile, and O, as two fp16 parts, behind the last, which also brings its columns into order.  As butterflies over registers they took as long as ten tiles: code that a
+// block runs once is fetched anew by every block, and that is what it costs.  (4 x 2048 queries on 4096 tokens: 645 us with butterflies in front, 568 so.)
+//
+// What bounds it.  Many rows: products and exponentials follow each other through S and P of a tile, and two tiles in flight, all that tensor memory holds, keep
+// the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 565 us, 973 TFLOP/s.  Few
+// rows, long sequences: the same chain for one tile, 2 x 16 queries on 65536 tokens, 64 heads on 8, 176 us, 793 GB/s of codes.  Short ones: what a block does
+// before its first tile and behind its last, 11 and 9 of 30 thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 21 us.
 //
 // Numbers are fp16 in the tensor core with fp32 sums, brought into fp16's range by powers of two: a query row by its largest element, the norms of
 // K and V by the largest of the tile.
@@ -44,7 +50,10 @@ constexpr int kCrossTile = 128;                      // tokens, query rows, padd
 constexpr int kCrossImage = kCrossTile * kCrossTile * 2;
 constexpr int kCrossTeam = 4;                        // warps that look up K, and as many for V
 constexpr int kCrossRowThreads = 384, kCrossThreads = kCrossRowThreads + 2 * kCrossTeam * 32;      // two warpgroups of rows, one of copies, norms and products; the teams
-constexpr int kCrossLaid = 2;                         // blocks of query rows a sequence from which on the images are laid out ahead
+// Tiles of query rows a sequence, on the average, above which the images are laid out ahead.  32 heads on 8, 8 sequences of 1500 tokens and 4 of 4096, bf16 results: 256 rows
+// 59.4 and 65.5 us laid out, 53.2 and 57.3 looked up, 512 rows 59.4 and 81.9, 63.5 and 86.0; fp16: 256 rows 55.3 and 71.6, 51.2 and 67.6, 512 rows 86.0 and 88.0,
+// 94.2 and 102.4.
+constexpr int kCrossLaid = 2;
 constexpr float kCrossRaise = 8.0f;                  // P up to 2^8
 constexpr double kCrossLevelScale = 1.42803;         // see tq_scored.cu
 constexpr float kCrossNoNorm = -1000.0f;             // the logarithm of V's scale in a tile whose V is all zero
@@ -1385,7 +1394,7 @@ static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, in
     const int64_t per = (exact ? 1 : 2) * kCrossTile, rows = (int64_t)total_q * (heads / kv_heads);
     l.items = rows / per + batch;                           // every sequence may end inside one
     l.kv_room = total_tokens / kCrossTile + batch;
-    l.laid = rows > kCrossLaid * per * batch;
+    l.laid = rows > (int64_t)kCrossLaid * kCrossTile * batch;
     // As many cuts of the tokens as fill the SMs, of two tiles (one a warpgroup) at least.
     const int64_t some = (rows + per - 1) / per, blocks = (some > batch ? some : batch) * kv_heads;
     const int64_t longest = (int64_t)max_pages * kPageTokens < total_tokens ? (int64_t)max_pages * kPageTokens : total_tokens;
