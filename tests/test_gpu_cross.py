@@ -112,6 +112,29 @@ def test_many_query_rows(q_lens, lens, Hq, H, D, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, out_dtype", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("D", [100, 128])
+def test_many_query_rows_of_other_types(D, dtype, out_dtype):
+    inputs, *got = run([300, 90], [260, 129], 8, 2, D, dtype=dtype, out_dtype=out_dtype)
+    check(inputs, *got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("q_lens", [[5, 30], [200, 100]])
+def test_rows_off_the_16_byte_boundary(q_lens, dtype):
+    """Views that begin an element behind a boundary: the same bits as from rows on it."""
+    cache, table, lens = paged([150, 300], 2, 128, 4)
+    q = torch.randn(sum(q_lens), 8, 128, generator=torch.Generator().manual_seed(0)).to(dtype).to(DEV)
+    cu = torch.tensor([0, *np.cumsum(q_lens)], dtype=torch.int32, device=DEV)
+    attn = TurboQuantPagedAttention(8, 128, 0.1, 2)
+    args = cu, cache.to(DEV), table.to(DEV), lens.to(DEV), 450
+    off_q, off_out = (torch.empty(q.numel() + 1, dtype=dtype, device=DEV)[1:].view(q.shape) for _ in range(2))
+    off_q.copy_(q)
+    assert torch.equal(attn.cross(q, *args), attn.cross(off_q, *args, off_out))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_many_query_rows_out_of_range(dtype):
     """Bad lengths, pages and a number of tokens that is too small: those sequences are left out and counted, the others are as they were."""
@@ -163,6 +186,8 @@ def test_rows_cut_over_blocks(q_lens, lens, H, dtype):
 @pytest.mark.gpu
 def test_many_sequences_spare_rows_and_tokens():
     inputs, *got = run([7, 0, 150] * 30, [90, 10, 0, 300, 129] * 18, 2, 1, more_rows=9, more_tokens=1000, width=30)
+    check(inputs, *got)
+    inputs, *got = run([3, 0, 1, 5] * 100, [40, 0, 129, 16, 1] * 80, 2, 1, more_rows=1)      # more than a lane's share of the search
     check(inputs, *got)
 
 

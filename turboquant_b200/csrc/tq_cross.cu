@@ -92,43 +92,71 @@ __device__ __forceinline__ int cross_qlen(const CrossParams& p, int b, bool& bad
     bad = c0 < 0 || c1 < c0 || c1 > p.total_q;
     return bad ? 0 : c1 - c0;
 }
+__device__ __forceinline__ int cross_upto(int v, int lane) {      // the sum of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
 // The sequence that item `index` of a kind belongs to (0: tiles of tokens; 1, 2: that many tiles of query rows); false: there are not so many.  A sequence
 // without queries has no tiles of tokens; one that ends behind the tiles which the caller's number of tokens makes has no tokens.  A whole warp.
 template <int KIND>
-__device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, int lane, CrossSeq& s, int* faults = nullptr) {
+__device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, int lane, CrossSeq& s) {
+    constexpr int kAhead = 4;                         // 32 sequences each, whose numbers are on their way together
     int64_t kv = 0, items = 0;
-    for (int base = 0; base < p.f.batch; base += 32) {
-        int len = 0, qlen = 0, kt = 0, mine = 0;
-        if (base + lane < p.f.batch) {
-            bool bad_len, bad_q;
-            len = cross_len(p, base + lane, bad_len);
-            qlen = cross_qlen(p, base + lane, bad_q);
-            kt = qlen > 0 ? (len + kCrossTile - 1) / kCrossTile : 0;
-            mine = KIND == 0 ? kt : (qlen * p.f.real_group + KIND * kCrossTile - 1) / (KIND == 0 ? 1 : KIND * kCrossTile);
-            if (faults) *faults += bad_len + bad_q;
-        }
-        int kt_to = kt, to = mine;
+    for (int base = 0; base < p.f.batch; base += 32 * kAhead) {
+        int len[kAhead], qlen[kAhead];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, kt_to, o), c = __shfl_up_sync(0xffffffffu, to, o);
-            if (lane >= o) { kt_to += a; to += c; }
+        for (int e = 0; e < kAhead; e++) {
+            const int b = base + 32 * e + lane;
+            bool bad;
+            len[e] = b < p.f.batch ? cross_len(p, b, bad) : 0;
+            qlen[e] = b < p.f.batch ? cross_qlen(p, b, bad) : 0;
         }
-        const bool kv_fits = kv + kt_to <= p.kv_room;
-        if (faults) *faults += kt > 0 && !kv_fits;
-        const uint32_t hit = __ballot_sync(0xffffffffu, index < items + to);
+        bool hit = false;
+        int kt = 0, mine = 0;
+#pragma unroll
+        for (int e = 0; e < kAhead; e++) {
+            if (hit || base + 32 * e >= p.f.batch) continue;
+            s.b = base + 32 * e;
+            s.len = len[e];
+            s.qlen = qlen[e];
+            kt = s.qlen > 0 ? (s.len + kCrossTile - 1) / kCrossTile : 0;
+            mine = KIND == 0 ? kt : (s.qlen * p.f.real_group + KIND * kCrossTile - 1) / (KIND == 0 ? 1 : KIND * kCrossTile);
+            const int all = __reduce_add_sync(0xffffffffu, mine);
+            hit = index < items + all;
+            if (!hit) {
+                items += all;
+                kv += __reduce_add_sync(0xffffffffu, kt);
+            }
+        }
         if (hit) {
-            const int l = __ffs(hit) - 1;
-            s.b = base + l;
+            const int to = cross_upto(mine, lane), l = __ffs(__ballot_sync(0xffffffffu, index < items + to)) - 1;
+            const int64_t kv_to = kv + cross_upto(kt, lane);
+            s.b += l;
             s.local = (int)(index - items) - __shfl_sync(0xffffffffu, to - mine, l);
-            s.len = __shfl_sync(0xffffffffu, kv_fits ? len : 0, l);
-            s.qlen = __shfl_sync(0xffffffffu, qlen, l);
-            s.kv0 = (int)(kv + __shfl_sync(0xffffffffu, kt_to - kt, l));
+            s.len = __shfl_sync(0xffffffffu, kv_to <= p.kv_room ? s.len : 0, l);
+            s.qlen = __shfl_sync(0xffffffffu, s.qlen, l);
+            s.kv0 = (int)__shfl_sync(0xffffffffu, kv_to - kt, l);
             return true;
         }
-        kv += __shfl_sync(0xffffffffu, kt_to, 31);
-        items += __shfl_sync(0xffffffffu, to, 31);
     }
     return false;
+}
+// Counts what is left out.  A whole warp, of one block.
+__device__ __forceinline__ void cross_count_faults(const CrossParams& p, int lane) {
+    int64_t kv = 0;
+    int faults = 0;
+    for (int base = 0; base < p.f.batch; base += 32) {
+        bool bad_len = false, bad_q = false;
+        const int b = base + lane, len = b < p.f.batch ? cross_len(p, b, bad_len) : 0, qlen = b < p.f.batch ? cross_qlen(p, b, bad_q) : 0;
+        const int kt = qlen > 0 ? (len + kCrossTile - 1) / kCrossTile : 0, to = cross_upto(kt, lane);
+        faults += bad_len + bad_q + (kt > 0 && kv + to > p.kv_room);
+        kv += __shfl_sync(0xffffffffu, to, 31);
+    }
+    if (faults) atomicAdd(&g_cross_faults, faults);
 }
 
 // Byte of 16-byte piece c (0 ... 15) of row r in an image: two halves of 128 rows x 128 bytes, the pieces of a row swizzled within its half.
@@ -198,12 +226,7 @@ __global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid
     grid_launch_dependents();
     for (int i = tid; i < 256 * 32; i += kLayThreads) lut[i] = (uint32_t)p.level_h[(i >> 5) & 15] | ((uint32_t)p.level_h[i >> 9] << 16);
     grid_dependency_wait();
-    if (blockIdx.x == 0 && warp == 0) {               // what is left out is counted once
-        CrossSeq s;
-        int faults = 0;
-        cross_find<0>(p, (int64_t)1 << 60, lane, s, &faults);
-        if (faults) atomicAdd(&g_cross_faults, faults);
-    }
+    if (blockIdx.x == 0 && warp == 0) cross_count_faults(p, lane);
     if (blockIdx.x == gridDim.x - 1) {                // the matrices of the way back and in
         const uint32_t one = p.f.q_dtype == TQ_BF16 ? 0x3F803F80u : 0x3C003C00u, negative = cross_negative(p.f.signs, tid & 15);
         for (int i = tid; i < kCrossTile * 16; i += kLayThreads) {
@@ -484,12 +507,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         }
     }
     grid_dependency_wait();
-    if (!LAID && blockIdx.x == 0 && warp == 8) {      // what is left out is counted once
-        CrossSeq none;
-        int faults = 0;
-        cross_find<0>(p, (int64_t)1 << 60, lane, none, &faults);
-        if (faults) atomicAdd(&g_cross_faults, faults);
-    }
+    if (!LAID && blockIdx.x == 0 && warp == 10) cross_count_faults(p, lane);
     if (!LAID && warp == 13) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {

@@ -276,9 +276,9 @@ class TurboQuantPagedAttention:
         the others, those of the largest ``scores`` (fp32 [batch, kv_heads, tokens], as ``decode_scored`` accumulates them), ``keep`` in
         all or the whole sequence where it is shorter; a tie goes to the lower position, a NaN counts as -inf.  What stays keeps
         its order and moves to positions 0, 1, ... of the pages of ``out_block_table`` (pages that the call does not read, so that
-        shared pages stay as they are), or of the sequence's own pages (None); the scores go with it to ``out_scores`` (None: in
-        place).  Returns ``(kept, lens)``: the positions that the tokens had, int32 [batch, kv_heads, keep], -1 behind the last one, and the new
-        lengths, int32 [batch].  Slots and scores behind them are left as they were."""
+        shared pages stay as they are), or of the sequence's own pages (None: no other sequence may then have them); the scores go
+        with it to ``out_scores`` (None: in place).  Returns ``(kept, lens)``: the positions that the tokens had, int32 [batch, kv_heads, keep],
+        -1 behind the last one, and the new lengths, int32 [batch].  Slots and scores behind them are left as they were."""
         done = self._calls.evict(kv_cache, block_table, seq_lens, scores, keep, recent, out_block_table, out_scores)
         if done is not None:
             return done
