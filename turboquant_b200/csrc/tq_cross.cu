@@ -19,8 +19,8 @@
 // come (43 us looked up, 53 laid out ahead, with 32 queries).
 //
 // S, then P, and O of two tiles are all of tensor memory: 2 x (128 + 128) columns.  With two tiles of query rows each warpgroup has one, and while it works out
-// exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn, and the first joins the second's
-// sums to its own at the end.  The running maximum is raised only when a logit exceeds it by 2^8, which makes rescaling O rare; a row needs no other
+// exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn, and at
+// the end each brings its O to the larger of their maxima and the product that rotates back adds them.  The running maximum is raised only when a logit exceeds it by 2^8, which makes rescaling O rare; a row needs no other
 // thread but its own.  Where few rows have long sequences the tokens are cut over several blocks as well, whose rows a second kernel joins.
 //
 // The rotations are matrix products too, with a matrix of ones and minus ones, exact in any type: the queries go through the tensor core as they come before the
@@ -68,7 +68,7 @@ struct CrossParams {
     float2* tile_scales;        // [tile][head]: K's power of two, the logarithm of V's
     uint16_t* tile_norms;       // exact: [tile][head][K, V][128]
     int64_t kv_room;            // tiles that there is room for
-    float* partial_o;           // [split][query row][query head][128], rotated domain
+    float* partial_o;           // [cut][group][query row][query head][128], rotated domain
     float* partial_lse;
     int total_q, splits;
     uint16_t level_h[16];
@@ -436,8 +436,7 @@ struct CrossMap {
     // has been handed over, so nobody reads the norms of tile t - 4 any more.
     static constexpr uint32_t kNorms = kImg + kImages * kCrossImage;
     static constexpr int kNormBytes = EXACT ? 2 * kCrossTile * 2 : LAID ? 0 : 2 * kCrossTile * 4;
-    static constexpr uint32_t kNormsEnd = kNorms + (kCrossMetas * kNormBytes > kCrossTile * 16 ? kCrossMetas * kNormBytes : kCrossTile * 16);      // (behind the last: sums of a group)
-    static constexpr size_t kSmem = kNormsEnd - 1024;
+    static constexpr size_t kSmem = kNorms + kCrossMetas * kNormBytes - 1024;
     static_assert(kSigns + 16 <= (LAID ? kQ : kCrossLut) && kSmem <= 232448 && kCrossUnit % 128 == 0, "shared memory of a block");
 };
 
@@ -949,17 +948,18 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                     __syncwarp();
                 }
             }
-            if (ok && p.splits == 1) {                // the way back: the two parts of O's rows, in S's place, against the matrix in V's
+            if (ok && p.splits == 1) {                // the way back: two parts of O's rows, in S's place, against the matrix in V's; of one tile, both groups' O
                 ok = image_there(k_item(n), 1);
-                for (int i = 0; i < (solo ? 1 : 2) && ok; i++) {
+                for (int i = 0; i < (solo && n == 1 ? 1 : 2) && ok; i++) {
                     ok = cross_wait(a_full + 8 * i, 0, gone);
                     tc_fence_after();
                     if (ok && elect_one()) {
-                        const uint64_t turn = cross_desc(M::kImg + (uint32_t)(k_item(n) % M::kImages) * kCrossImage);
+                        const uint64_t turn = img_desc + (uint64_t)(k_item(n) % M::kImages) * kImage16;
+                        const int to = solo ? 0 : i;
 #pragma unroll 1
                         for (int kk = 0; kk < 16; kk++)
-                            mq_mma_ts(256 + 128 * i, 128 * i + 8 * kk, turn + (uint64_t)(((kk >> 2) & 1) * 1024 + (kk & 3) * 2), idesc, kk ? 1u : 0u);
-                        cross_commit(d_full + 8 * i);
+                            mq_mma_ts(256 + 128 * to, 128 * i + 8 * kk, turn + (uint64_t)(((kk >> 2) & 1) * 1024 + (kk & 3) * 2), idesc, kk || to != i ? 1u : 0u);
+                        if (!solo || i == 1 || n == 1) cross_commit(d_full + 8 * to);
                     }
                     __syncwarp();
                 }
@@ -1190,52 +1190,82 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             __syncwarp();
             if (lane == 0) cross_arrive(p_full + 8 * i);
         }
-        // ---- the row: joined, normalized, rotated back, out; or a partial ----------------------------------
-        if (ok && turns > 0) ok = cross_wait(o_full + 8 * i, 0, gone);
+        // ---- the row: normalized, brought back, out or to the partials ---------------------------------
+        if (ok && n > 0) ok = cross_wait(o_full + 8 * (turns > 0 ? i : 0), 0, gone);
         if (!ok) *gone = 1;
         tc_fence_after();
-        // O of the row is in units of 2^ev_ref; with a second group's sums, brought over in images that are free, in units of the larger.
-        const bool joined = solo && n > 1;
-        float scale = 1.0f, scale_other = 0.0f;
-        // (the two images that are not the matrix of the way back: 64 rows each)
-        const uint32_t joint = M::kImg + (uint32_t)((k_item(n) + 1 + (r >> 6)) % M::kImages) * kCrossImage + (uint32_t)(r & 63) * kCrossTile * 4;
-        if (joined) {
-            float4* const sums = reinterpret_cast<float4*>(window + M::kNorms);
-            if (i == 1) {                             // once the first group's products are done with the images too
-                if (ok) ok = cross_wait(o_full, 0, gone);
-                if (ok) {
+        // O of the row is in units of 2^ev_ref; one tile's two groups bring theirs to the larger.  (What is written to the queries' place: by now all S are formed.)
+        float scale = 1.0f;
+        const bool cut = p.splits > 1;
+        if (solo && n > 0 && !cut) {
+            float4* const sums = reinterpret_cast<float4*>(window + M::kQ);
+            sums[tid] = make_float4(m, l, ev_ref, 0.0f);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float4 other = sums[tid ^ 128];
+            const float mm = fmaxf(m, other.x), ev = fmaxf(ev_ref, other.z), c0 = fast_exp2(m - mm);
+            scale = c0 * fast_exp2(ev_ref - ev);
+            l = l * c0 + other.y * fast_exp2(other.x - mm);
+            m = mm;
+            ev_ref = ev;
+            if (*gone) ok = false;
+        }
+        if (__all_sync(0xffffffffu, ok)) {
+            const bool none = l == 0.0f, live = row < rows;
+            const float unit = p.f.v_scale * fast_exp2(ev_ref);
+            const int qi = row / G, g = row - qi * G;
+            const int64_t to = live ? (int64_t)(q_first + qi) * p.f.real_heads + h * G + g : -1;
+            const float lse2 = none ? -INFINITY : m + log2f(l);
+            if (cut) {
+                // A partial of the group's own, as O has its columns.  There are two for each cut; rows that one group has to itself leave the other empty.
+                const int64_t part = (int64_t)p.total_q * p.f.real_heads, at = (2 * split + (solo ? i : 0)) * part + to;
+                if (live) {
+                    p.partial_lse[at] = lse2;
+                    if (!solo) p.partial_lse[at + part] = -INFINITY;
+                }
+                scale = unit / l;
 #pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        float v[32];
-                        cross_ld(tm_o + 32 * c, v);
-                        cross_ld_wait(v);
+                for (int c = 0; c < 4 && turns > 0; c++) {
+                    float v[32];
+                    __syncwarp();
+                    cross_ld(tm_o + 32 * c, v);
+                    cross_ld_wait(v);
+                    float4* const dst = reinterpret_cast<float4*>(p.partial_o + at * kCrossTile + 32 * c);
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            cross_sts(joint + 16 * ((8 * c + e) ^ (r & 7)), __float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
-                    }
-                    sums[r] = make_float4(m, l, ev_ref, 0.0f);
+                    for (int e = 0; e < 8; e++)
+                        if (live && !none) dst[e] = make_float4(v[4 * e] * scale, v[4 * e + 1] * scale, v[4 * e + 2] * scale, v[4 * e + 3] * scale);
                 }
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (i == 0) {
-                const float4 other = sums[r];
-                const float mm = fmaxf(m, other.x), ev = fmaxf(ev_ref, other.z), c0 = fast_exp2(m - mm), c1 = fast_exp2(other.x - mm);
-                scale = c0 * fast_exp2(ev_ref - ev);
-                scale_other = c1 * fast_exp2(other.z - ev);
-                m = mm;
-                l = l * c0 + other.y * c1;
-                ev_ref = ev;
+            if (turns > 0 && !cut) {
+                // The weighted mean as two fp16 parts in S's place (at most 2^15: a mean of rows of levels below 4 times norms below 2^7, under powers of two up to
+                // 2^6).
+                scale *= none ? 0.0f : 1.0f / l;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    float v[32];
+                    cross_ld(tm_o + 32 * c, v);
+                    cross_ld_wait(v);
+                    uint32_t a[16], b[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float x = none ? 0.0f : v[2 * e] * scale, y = none ? 0.0f : v[2 * e + 1] * scale;
+                        a[e] = pack_half2(x, y);
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&a[e]));
+                        b[e] = pack_half2(x - back.x, y - back.y);
+                    }
+                    cross_st16(tm_s + 16 * c, a);
+                    cross_st16(tm_s + 64 + 16 * c, b);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) cross_arrive(a_full + 8 * i);
             }
-        }
-        if (__all_sync(0xffffffffu, ok && !(solo && i == 1) && !(joined && *gone))) {
-            const bool none = l == 0.0f, live = row < rows, cut = p.splits > 1;
-            const float inv = none ? 0.0f : 1.0f / l, lse2 = none ? -INFINITY : m + log2f(l), unit = p.f.v_scale * fast_exp2(ev_ref);
-            scale *= inv;
-            scale_other *= inv;
-            const int qi = row / G, g = row - qi * G;
-            const int64_t to = live ? (int64_t)(q_first + qi) * p.f.real_heads + h * G + g : -1, at = (int64_t)split * p.total_q * p.f.real_heads + to;
-            // 64 bytes each of the warp's rows go to memory by way of shared memory (the queries' place), neighbouring lanes to neighbouring pieces of a row.
-            const uint32_t stage = M::kQ + i * kCrossImage + (warp & 3) * 2048;
+            if (p.f.out_lse && live && !cut && !(solo && i == 1)) p.f.out_lse[to] = lse2 * 0.6931471805599453f;
+            const int mine = solo ? 0 : i;            // whose O's place the result is in
+            if (n > 0 && !cut) ok = cross_wait(d_full + 8 * mine, 0, gone);
+            tc_fence_after();
+            // 64 bytes each of the warp's rows go to memory by way of shared memory, neighbouring lanes to neighbouring pieces of a row.
+            const uint32_t stage = M::kQ + 4096 + warp * 2048;
             auto place = [&](int row, int piece) { return stage + row * 64 + 16 * (piece ^ ((row >> 1) & 3)); };
             auto rows_out = [&](const uint32_t* v, int at_byte) {
                 __syncwarp();
@@ -1250,95 +1280,38 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                     if (row_to >= 0 && at_byte + 16 * piece < 2 * D) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.f.out) + row_to * 2 * D + at_byte + 16 * piece) = x;
                 }
             };
-            // The weighted mean, columns as O has them: a partial, or two fp16 parts in S's place for the way back (at most 2^15: a mean of rows of levels below 4 times
-            // norms below 2^7, under powers of two up to 2^6).
+            const bool whole = p.f.out_dtype != TQ_F32 && D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f.out) & 15) == 0;
+            const float f = unit * p.f.scale;
 #pragma unroll 1
-            for (int c = 0; c < 4; c++) {
+            for (int c = solo ? 2 * i : 0; c < (solo ? 2 * i + 2 : 4) && ok && !cut; c++) {
                 float v[32];
-                if (turns > 0) {
-                    cross_ld(tm_o + 32 * c, v);
+                __syncwarp();
+                if (n > 0) {
+                    cross_ld(tmem + 256 + 128 * mine + lane_at + 32 * c, v);
                     cross_ld_wait(v);
                 }
-                if (joined) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float4 o = cross_lds_f4(joint + 16 * ((8 * c + e) ^ (r & 7)));
-                        v[4 * e] = v[4 * e] * scale + o.x * scale_other; v[4 * e + 1] = v[4 * e + 1] * scale + o.y * scale_other;
-                        v[4 * e + 2] = v[4 * e + 2] * scale + o.z * scale_other; v[4 * e + 3] = v[4 * e + 3] * scale + o.w * scale_other;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] *= scale;
-                }
-                if (none) {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = 0.0f;
-                }
-                if (cut) {
-                    if (live) {
-                        float4* const dst = reinterpret_cast<float4*>(p.partial_o + at * kCrossTile + 32 * c);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) dst[e] = make_float4(v[4 * e] * unit, v[4 * e + 1] * unit, v[4 * e + 2] * unit, v[4 * e + 3] * unit);
-                    }
-                    __syncwarp();
-                } else if (n > 0) {
-                    uint32_t a[16], b[16];
+                for (int e = 0; e < 32; e++) v[e] = none ? 0.0f : v[e] * f;
+                if (whole) {
+                    uint32_t u[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        a[e] = pack_half2(v[2 * e], v[2 * e + 1]);
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&a[e]));
-                        b[e] = pack_half2(v[2 * e] - back.x, v[2 * e + 1] - back.y);
-                    }
-                    cross_st16(tm_s + 16 * c, a);
-                    cross_st16(tm_s + 64 + 16 * c, b);
-                }
-            }
-            if (live) {
-                if (cut) p.partial_lse[at] = lse2;
-                else if (p.f.out_lse) p.f.out_lse[to] = lse2 * 0.6931471805599453f;
-            }
-            if (!cut) {
-                if (n > 0) {
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) cross_arrive(a_full + 8 * i);
-                    ok = cross_wait(d_full + 8 * i, 0, gone);
-                    tc_fence_after();
-                }
-                const bool whole = p.f.out_dtype != TQ_F32 && D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f.out) & 15) == 0;
-                const float f = unit * p.f.scale;
-#pragma unroll 1
-                for (int c = 0; c < 4 && ok; c++) {
-                    float v[32];
-                    __syncwarp();
-                    if (n > 0) {
-                        cross_ld(tm_o + 32 * c, v);
-                        cross_ld_wait(v);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = none ? 0.0f : v[e] * f;
-                    if (whole) {
-                        uint32_t u[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            if (p.f.out_dtype == TQ_BF16) {
-                                const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                                u[e] = *reinterpret_cast<const uint32_t*>(&t);
-                            } else {
-                                u[e] = pack_half2(v[2 * e], v[2 * e + 1]);
-                            }
+                        if (p.f.out_dtype == TQ_BF16) {
+                            const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                            u[e] = *reinterpret_cast<const uint32_t*>(&t);
+                        } else {
+                            u[e] = pack_half2(v[2 * e], v[2 * e + 1]);
                         }
-                        rows_out(u, 64 * c);
-                    } else if (live) {
+                    }
+                    rows_out(u, 64 * c);
+                } else if (live) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            if (32 * c + e >= D) continue;
-                            const int64_t o = to * D + 32 * c + e;
-                            if (p.f.out_dtype == TQ_BF16) reinterpret_cast<__nv_bfloat16*>(p.f.out)[o] = __float2bfloat16_rn(v[e]);
-                            else if (p.f.out_dtype == TQ_F16) reinterpret_cast<__half*>(p.f.out)[o] = __float2half_rn(v[e]);
-                            else reinterpret_cast<float*>(p.f.out)[o] = v[e];
-                        }
+                    for (int e = 0; e < 32; e++) {
+                        if (32 * c + e >= D) continue;
+                        const int64_t o = to * D + 32 * c + e;
+                        if (p.f.out_dtype == TQ_BF16) reinterpret_cast<__nv_bfloat16*>(p.f.out)[o] = __float2bfloat16_rn(v[e]);
+                        else if (p.f.out_dtype == TQ_F16) reinterpret_cast<__half*>(p.f.out)[o] = __float2half_rn(v[e]);
+                        else reinterpret_cast<float*>(p.f.out)[o] = v[e];
                     }
                 }
             }
@@ -1359,6 +1332,8 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
     grid_launch_dependents();
     grid_dependency_wait();
     if (at >= rows) return;
+    const int parts = 2 * p.splits;
+    float lse = lane < parts ? p.partial_lse[lane * rows + at] : -INFINITY;      // of the first 32 parts, a lane each
     // a row that belongs to no sequence, or to one that was left out, is left as it is
     const int t = (int)(at / p.f.real_heads);
     bool live = false;
@@ -1368,15 +1343,24 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
         live = __any_sync(0xffffffffu, in);
     }
     if (!live) return;
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.partial_lse[s * rows + at]);
-    if (m == -INFINITY) m = 0.0f;
-    for (int s = 0; s < p.splits; s++) {
-        const float w = fast_exp2(p.partial_lse[s * rows + at] - m);
-        l += w;
-        const float* const v = p.partial_o + (s * rows + at) * kCrossTile + 64 * (lane & 1) + (lane >> 1);      // dim 8 w + d is column 16 d + w
+    float m = lse, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 32 + lane; s < parts; s += 32) m = fmaxf(m, p.partial_lse[s * rows + at]);
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = fmaf(w, v[16 * e], o[e]);
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int base = 0; base < parts; base += 32) {
+        if (base > 0) lse = base + lane < parts ? p.partial_lse[(base + lane) * rows + at] : -INFINITY;
+        const float mine = lse == -INFINITY ? 0.0f : fast_exp2(lse - m);
+#pragma unroll 4
+        for (int s = 0; s < min(32, parts - base); s++) {
+            const float w = __shfl_sync(0xffffffffu, mine, s);
+            const float* const v = p.partial_o + ((base + s) * rows + at) * kCrossTile + 64 * (lane & 1) + (lane >> 1);      // dim 8 w + d is column 16 d + w
+            l += w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float x = v[16 * e];
+                if (w != 0.0f) o[e] = fmaf(w, x, o[e]);      // (else nothing has been written there)
+            }
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -1424,7 +1408,7 @@ static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, in
     l.scales = l.turn + (l.laid ? 2 * kCrossImage : 0);
     l.norms = l.scales + cross_up(units * sizeof(float2));
     l.partial_lse = l.norms + (exact ? cross_up(units * 2 * kCrossTile * 2) : 0);
-    const size_t cut = l.splits > 1 ? (size_t)l.splits * total_q * heads : 0;
+    const size_t cut = l.splits > 1 ? (size_t)2 * l.splits * total_q * heads : 0;
     l.partial_o = l.partial_lse + cross_up(cut * 4);
     l.end = l.partial_o + cross_up(cut * kCrossTile * 4);
     return l;
