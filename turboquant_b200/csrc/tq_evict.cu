@@ -7,23 +7,25 @@
 //
 //   select   A cluster of blocks for each (sequence, head) finds the score of rank k = keep - recent by its bits from the top.  A score becomes an
 //            unsigned word that sorts as the float does.  The leading eleven bits (sign, exponent, two of the fraction) come from a histogram of all
-//            tokens, summed over the cluster through distributed shared memory; a second walk over the tokens counts those above that bin
-//            and lists those in it, a few in a hundred; the other bits, 8, 8 and 5 at a time, come from the lists.  Then the counts of what stays
-//            are summed over the warps and blocks in front, each of which has a run of tokens of its own, and in a third walk
-//            every warp writes its tokens at consecutive places.  No order of atomics reaches the result.
+//            tokens, summed over the cluster through distributed shared memory; a second walk over the tokens counts those above that bin,
+//            lists those in it, a few in a hundred, and the places of both; the other bits, 8, 8 and 5 at a time, come from the lists.  Then the counts of what stays
+//            are summed over the warps and blocks in front, each of which has a run of tokens of its own, and from the places (or a
+//            third walk, where there are too many) every warp writes its tokens one behind the other (a million tokens, 1 in 16 stays: 124 us with
+//            the third walk, 112 so; 1 in 4 of 32768, keys in shared memory: 66.5 and 67.2).  No order of atomics reaches the result.
 //   move     A block for each page of the destination: all its slots of K and V, 16 bytes a thread and step, so that the stores cover
 //            whole lines; the loads are gathered slots.
 //
 // What bounds it: the scores are read once (4 bytes a token and head), the kept slots are read and written (160 bytes each way for a
 // head of 128).  Memory is read in 64-byte pieces, of which a slot of 80 bytes anywhere touches 2.2: the move of 8 sequences' 8192 tokens of 32768,
 // 8 heads, takes 45 us for 166 MB read and 84 MB written, 5.5 TB/s; the selection before it 21 us, the walks of 16384 scores by 16 warps an SM
-// and the cluster's waits between them.  One sequence of a million tokens, 8 heads: 124 us, the selection 75 of them, as a cluster has no more than 16 SMs for a head.
+// and the cluster's waits between them.  One sequence of a million tokens, 8 heads: 112 us, the selection 63 of them, as a cluster has no more than 16 SMs for a head and
+// issues 60 percent of their slots.
 #include "tq_common.cuh"
 
 namespace tq {
 
-// Threads of a block of the selection: two blocks an SM; or one, where its share has no room in shared memory and each walk over it waits for L2 (a million tokens, 8 heads:
-// 138 us with 512 threads a block, 124 with 1024; shares of 16384 tokens in shared memory: 66.5 and 66.9).
+// Threads of a block of the selection: two blocks an SM; or one, where its share has no room in shared memory and each walk over it waits for L2 (a million
+// tokens, 8 heads, three walks: 138 us with 512 threads a block, 124 with 1024; shares of 16384 tokens in shared memory: 66.5 and 66.9).
 constexpr int kEvictThreads = 512, kEvictManyThreads = 1024;
 constexpr int kEvictRun = 128;                 // tokens of a warp's load: four a lane
 constexpr int kEvictAhead = 4;                 // loads in flight together
@@ -33,6 +35,7 @@ constexpr int kEvictMaxCluster = 16;
 constexpr int kEvictBins = 2048, kEvictColumns = 8, kEvictDigits = 256;
 constexpr int kEvictHistBytes = kEvictBins * kEvictColumns * 4, kEvictDigitBytes = kEvictDigits * 32 * 4;
 constexpr int kEvictListBytes = kEvictHistBytes - kEvictDigitBytes;
+constexpr int kEvictMost = 221184, kEvictHalf = 104448;      // shared memory of one block an SM, of two, without the fixed arrays
 constexpr int kEvictMostKeys = 36 * 1024;      // sort keys a block keeps in shared memory beside them; longer shares are read from L2 in every walk
 
 struct EvictParams {
@@ -50,6 +53,7 @@ struct EvictParams {
     int64_t score_b, score_h, to_b, to_h, out_b, out_h;
     int batch, kv_heads, slot_bytes, max_pages, out_max_pages, out_pages, max_tokens, keep, recent, cluster, wide;
     int scores_staged;
+    int listed;                    // places that a warp has for its tokens that may stay
 };
 
 static __device__ int32_t g_evict_faults = 0;
@@ -113,7 +117,7 @@ __global__ void __launch_bounds__(KEPT ? kEvictThreads : kEvictManyThreads, KEPT
     extern __shared__ __align__(16) uint32_t evict_smem[];
     uint32_t* const hist = evict_smem;                            // [bin][column], then [digit][lane]
     uint32_t* const lists = evict_smem + kEvictDigitBytes / 4;
-    uint32_t* const keys = evict_smem + kEvictHistBytes / 4;      // the block's share, KEPT
+    uint32_t* const keys = evict_smem + kEvictHistBytes / 4;      // the block's share, KEPT; behind it the places of tokens that may stay
     __shared__ __align__(16) int sums[kEvictBins], sums8[2][kEvictDigits];
     __shared__ int counts[2], warp_gt[32], warp_eq[32], found[2][2], above_s[2][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -158,6 +162,7 @@ __global__ void __launch_bounds__(KEPT ? kEvictThreads : kEvictManyThreads, KEPT
     const int64_t begin64 = ((int64_t)rank * kWarps + warp) * W;
     const int begin = begin64 < M ? (int)begin64 : M, end = begin64 + W < M ? (int)(begin64 + W) : M;
     uint32_t* const my_keys = keys + (size_t)warp * W;
+    uint16_t* const mays = reinterpret_cast<uint16_t*>(keys + (KEPT ? (size_t)kWarps * W : 0)) + (size_t)warp * p.listed;
     const bool wide = p.wide;
     // Goes over the warp's tokens, four a lane in each of kEvictAhead runs: body(first token of the lane in a run, keys, a run).  Past the end the key is zero, which
     // no score has.
@@ -263,10 +268,27 @@ __global__ void __launch_bounds__(KEPT ? kEvictThreads : kEvictManyThreads, KEPT
     // ---- what lies above, and the list of what lies in the bin ---------------------------------------------
     const uint32_t lower = (1u << lane) - 1u;
     uint32_t* const list = lists + warp * kList;
-    int gt = 0, listed = 0;
-    walk(true, [&](int, const uint32_t (&key)[4]) {
+    int gt = 0, listed = 0, may = 0;
+    walk(true, [&](int at, const uint32_t (&key)[4]) {
+        // those in the bin or above it, by position: what the last walk has to look at
+        uint32_t mine = 0, below = 0, all = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) gt += key[e] >> 21 > prefix;
+        for (int e = 0; e < 4; e++) {
+            gt += key[e] >> 21 > prefix;
+            const bool stays = key[e] >> 21 >= prefix && key[e] != 0u;
+            const uint32_t m = __ballot_sync(0xffffffffu, stays);
+            mine |= (uint32_t)stays << e;
+            below += __popc(m & lower);
+            all += __popc(m);
+        }
+        int place = may + (int)below;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (mine >> e & 1u) {
+                if (place < p.listed) mays[place] = (uint16_t)(at + e - begin);
+                place++;
+            }
+        may += (int)all;
         const bool in[4] = {key[0] >> 21 == prefix && key[0] != 0u, key[1] >> 21 == prefix && key[1] != 0u, key[2] >> 21 == prefix && key[2] != 0u,
                             key[3] >> 21 == prefix && key[3] != 0u};
         if (__any_sync(0xffffffffu, in[0] | in[1] | in[2] | in[3])) {
@@ -402,6 +424,35 @@ __global__ void __launch_bounds__(KEPT ? kEvictThreads : kEvictManyThreads, KEPT
     leave();
     int ties = left - before_eq;       // of this warp's tokens with the key of rank k, the first `ties` stay
     int place = before_gt + min(before_eq, left);
+    if (may <= p.listed) {
+        __syncwarp();
+        for (int i = 0; i < may; i += 32) {
+            const bool in = i + lane < may;
+            const int at = begin + (in ? (int)mays[i + lane] : 0);
+            uint32_t key = 0;
+            float score = 0.0f;
+            if constexpr (KEPT) {
+                key = in ? my_keys[at - begin] : 0u;
+                score = __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+                if (key == 0x80000000u || key == 0x007fffffu) score = row[at];      // a key that stands for two (zeros, a NaN and -inf)
+            } else if (in) {
+                score = row[at];
+                key = evict_key(score);
+            }
+            const bool is_eq = key == prefix;
+            const uint32_t same = __ballot_sync(0xffffffffu, is_eq);
+            const bool stays = key > prefix || (is_eq && __popc(same & lower) < ties);
+            const uint32_t m = __ballot_sync(0xffffffffu, stays);
+            if (stays) {
+                const int j = place + __popc(m & lower);
+                kept[j] = at;
+                to[j] = score;
+            }
+            ties -= __popc(same);
+            place += __popc(m);
+        }
+        return;
+    }
     walk(true, [&](int at, const uint32_t (&key)[4]) {
         bool is_eq[4], stays[4];
 #pragma unroll
@@ -523,16 +574,16 @@ static size_t evict_up(size_t x) { return (x + 255) & ~(size_t)255; }
 template <bool KEPT>
 static int launch_select(EvictParams& p, int units, int C, int too_long, cudaStream_t s) {
     // (A cluster stays inside one of the device's groups of SMs, which have not all the same number: eight of sixteen blocks would run seven and one.)
-    static int active[64][kEvictMaxCluster + 1] = {};      // by device: clusters of c blocks that run at the same time, plus one
+    static int active[64][2][kEvictMaxCluster + 1] = {};      // by device, and one block an SM or two: clusters of c blocks that run at the same time, plus one
     int dev = 0;
     TQ_CUDA(cudaGetDevice(&dev));
     TQ_REQUIRE(dev >= 0 && dev < 64, TQ_ERR_UNSUPPORTED, "device %d", dev);
     const auto kernel = evict_select_kernel<KEPT>;
-    constexpr int THREADS = KEPT ? kEvictThreads : kEvictManyThreads, kMost = kEvictHistBytes + (KEPT ? kEvictMostKeys * 4 : 0);
-    if (active[dev][1] == 0) {
-        TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    constexpr int THREADS = KEPT ? kEvictThreads : kEvictManyThreads, kWarps = THREADS / 32;
+    if (active[dev][0][1] == 0) {
+        TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictMost));
         TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        active[dev][1] = 1;
+        active[dev][0][1] = 1;
     }
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(THREADS);
@@ -543,11 +594,14 @@ static int launch_select(EvictParams& p, int units, int C, int too_long, cudaStr
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    auto share = [&](int c) { return ((p.max_tokens + THREADS / 32 * c - 1) / (THREADS / 32 * c) + kEvictRun - 1) / kEvictRun * kEvictRun * (THREADS / 32); };
+    auto run = [&](int c) { return ((p.max_tokens + kWarps * c - 1) / (kWarps * c) + kEvictRun - 1) / kEvictRun * kEvictRun; };      // tokens of a warp
+    auto need = [&](int c) { return kEvictHistBytes + (KEPT ? (int64_t)run(c) * kWarps * 4 : 0); };
+    auto two = [&](int c) { return KEPT && need(c) <= kEvictHalf; };
     for (; C > 1; C--) {
-        if (active[dev][C] == 0) {
+        int& known = active[dev][two(C)][C];
+        if (known == 0) {
             cfg.gridDim = dim3((unsigned)(64 * C));
-            cfg.dynamicSmemBytes = KEPT ? kMost / 2 : kMost;      // (shares of up to a few thousand keys leave two an SM)
+            cfg.dynamicSmemBytes = two(C) ? kEvictHalf : kEvictMost;
             attr[0].val.clusterDim.x = (unsigned)C;
             cfg.numAttrs = 1;
             int n = 0;
@@ -555,14 +609,17 @@ static int launch_select(EvictParams& p, int units, int C, int too_long, cudaStr
                 cudaGetLastError();
                 n = 0;
             }
-            active[dev][C] = n + 1;
+            known = n + 1;
         }
-        if (active[dev][C] - 1 >= units) break;
+        if (known - 1 >= units) break;
     }
-    if (KEPT && share(C) > kEvictMostKeys) return too_long;
+    if (need(C) > kEvictHistBytes + kEvictMostKeys * 4) return too_long;
     p.cluster = C;
+    // What is left of the memory has the places of tokens that may stay; a warp with more of them walks over all its tokens.
+    const int room = (int)((two(C) ? kEvictHalf : kEvictMost) - need(C)) / 2 / kWarps;
+    p.listed = run(C) <= 65536 ? (run(C) < room ? run(C) : room) : 0;
     cfg.gridDim = dim3((unsigned)(units * C));
-    cfg.dynamicSmemBytes = KEPT ? kEvictHistBytes + (size_t)share(C) * 4 : (size_t)kMost;
+    cfg.dynamicSmemBytes = (size_t)need(C) + (size_t)p.listed * 2 * kWarps;
     attr[0].val.clusterDim.x = (unsigned)C;
     cfg.numAttrs = 2;
     TQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
