@@ -456,7 +456,6 @@ template <bool EXACT, bool LAID>
 __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cross_attend_kernel(const __grid_constant__ CrossParams p) {
     constexpr int kTiles = EXACT ? 1 : 2;             // of query rows
     using M = CrossMap<EXACT, LAID>;
-    constexpr int kThreads = LAID ? kCrossRowThreads : kCrossThreads;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, H = p.f.kv_heads, G = p.f.real_group;
     uint8_t* const window = smem - smem_u32(smem);    // address 0 of the block's window
@@ -498,26 +497,43 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         *gone = 0;
         fence_barrier_init();
     }
-    if (!LAID && warp >= 12) {                        // the table, ahead of the wait
+    if (!LAID && warp >= 12) {                        // the table, the matrix of the way in and the signs' bits, while the others look for the sequence
         const uint32_t mine = p.level_h[lane & 15];
         for (int v = 4 * (warp - 12) + (lane >> 3); v < 256; v += 8 * kCrossTeam) {
             const uint32_t e = __shfl_sync(0xffffffffu, mine, v & 15) | (__shfl_sync(0xffffffffu, mine, v >> 4) << 16);
             *reinterpret_cast<uint4*>(window + kCrossLut + v * 128 + 16 * (lane & 7)) = make_uint4(e, e, e, e);
         }
+        const int c = lane & 15;
+        const uint32_t one = p.f.q_dtype == TQ_BF16 ? 0x3F803F80u : 0x3C003C00u, negative = cross_negative(p.f.signs, c);
+#pragma unroll 1
+        for (int col = 2 * (warp - 12) + (lane >> 4); col < kCrossTile; col += 4 * kCrossTeam) {
+            const uint4 v = cross_way_in(col, c, negative, one);
+            cross_sts(M::kWay + cross_piece(col, c), v.x, v.y, v.z, v.w);
+        }
+        if (warp == 12 && lane < 16) (window + M::kSigns)[lane] = (uint8_t)negative;      // a byte every eight dims
+        fence_proxy_async();
     }
     grid_dependency_wait();
     if (!LAID && blockIdx.x == 0 && warp == 10) cross_count_faults(p, lane);
-    if (!LAID && warp == 13) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t negative = __ballot_sync(0xffffffffu, p.f.signs[32 * i + lane] < 0.0f);
-            if (lane == 0) reinterpret_cast<uint32_t*>(window + M::kSigns)[i] = negative;
-        }
-    }
     CrossSeq s;
     const int64_t item = blockIdx.x / p.splits;
     const int split = (int)(blockIdx.x - item * p.splits), h = (int)(item % H);
-    if (!cross_find<kTiles>(p, item / H, lane, s)) return;                // uniform over the block
+    if constexpr (LAID) {
+        if (!cross_find<kTiles>(p, item / H, lane, s)) return;            // uniform over the block
+    } else {
+        int* const told = reinterpret_cast<int*>(window + M::kBars + 416);
+        bool found = true;
+        if (warp < 12) found = cross_find<kTiles>(p, item / H, lane, s);
+        if (tid == 0) {
+            told[0] = found; told[1] = s.b; told[2] = s.local; told[3] = s.len; told[4] = s.qlen;
+        }
+        __syncthreads();
+        if (warp >= 12) {
+            found = told[0] != 0;
+            s.b = told[1]; s.local = told[2]; s.len = told[3]; s.qlen = told[4];
+        }
+        if (!found) return;                           // uniform over the block
+    }
     const int rows = s.qlen * G, row0 = s.local * kTiles * kCrossTile;
     const bool solo = kTiles == 1 || rows - row0 <= kCrossTile;           // one tile of query rows
     const int all = (s.len + kCrossTile - 1) / kCrossTile;
@@ -557,21 +573,21 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         if (lane < some)
             split_box(kCrossRaw + (ring8 + stage) * kCrossUnit + lane * kPageTokens * kSlotBytes, &p.f.cache_map, h * kSlotBytes, id * kPageTokens, which, bar);
     };
-    // The queries: 16-bit rows as they come into the images' place (asynchronous copies, all in flight together), and the matrix that rotates them.
     const int q_tiles = solo ? 1 : 2, q_rows = min(rows - row0, q_tiles * kCrossTile), q_first = p.cu_q[s.b];
     const bool halves = p.f.q_dtype != TQ_F32;
     auto row_of = [&](int r) -> int64_t {             // of the query tensor
         const int row = row0 + r, qi = row / G;
         return (int64_t)(q_first + qi) * p.f.real_heads + h * G + (row - qi * G);
     };
-    if (halves && n > 0) {
+    // As they come into the images' place, all in flight together, by the block's first `threads` threads.
+    auto load_queries = [&](int threads) {
+        if (!halves || n == 0) return;
         const uint16_t* const q16 = reinterpret_cast<const uint16_t*>(p.f.q);
         const bool whole = D % 8 == 0 && (reinterpret_cast<uintptr_t>(q16) & 15) == 0;
-        constexpr int kStep = kThreads / 16;          // rows on: a query row's place moves by on_q queries and on_g heads
-        const int c = tid & 15, on_q = kStep / G, on_g = kStep - on_q * G;
+        const int step = threads / 16, c = tid & 15, on_q = step / G, on_g = step - on_q * G;      // rows on: a query row's place moves by on_q queries and on_g heads
         int r = tid >> 4, qi = (row0 + r) / G, g = row0 + r - qi * G;
 #pragma unroll 1
-        for (; r < q_tiles * kCrossTile; r += kStep) {
+        for (; r < q_tiles * kCrossTile; r += step) {
             const int some = r < q_rows ? min(8, D - 8 * c) : 0;
             const uint32_t to = M::kQ + (r >> 7) * kCrossImage + cross_piece(r & 127, c);
             const uint16_t* const from = some > 0 ? q16 + ((int64_t)(q_first + qi) * p.f.real_heads + h * G + g) * D + 8 * c : q16;
@@ -590,22 +606,15 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 cross_sts(to, v[0], v[1], v[2], v[3]);
             }
         }
-        if constexpr (!LAID) {
-            const uint32_t one = p.f.q_dtype == TQ_BF16 ? 0x3F803F80u : 0x3C003C00u;
-            const uint32_t negative = cross_negative(p.f.signs, c);
-#pragma unroll 1
-            for (int col = tid >> 4; col < kCrossTile; col += kStep) {
-                const uint4 v = cross_way_in(col, c, negative, one);
-                cross_sts(M::kWay + cross_piece(col, c), v.x, v.y, v.z, v.w);
-            }
-        }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
+    };
+    if constexpr (LAID) {
+        load_queries(kCrossRowThreads);
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;                 // S / P of group i at 128 i, O at 256 + 128 i; all 512 columns: zero
 
     if (!LAID && warp >= 12) {
         const uint32_t lut_lane = kCrossLut + 4 * lane;
@@ -875,6 +884,10 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 for (int kk = 0; kk < 4; kk++) mq_mma_ts(256 + 128 * i, 128 * i + 32 * half + 8 * kk, v_desc + (uint64_t)(kk * 2), idesc, more || half || kk ? 1u : 0u);
             };
             auto image_there = [&](int item, int half) { return cross_wait(img_full + 16 * (item % M::kImages) + (LAID ? 8 : 8 * half), (item / M::kImages) & 1, gone); };
+            if constexpr (!LAID) {
+                tc_fence_before();
+                asm volatile("bar.sync 3, 288;" ::: "memory");     // the rows' warps have the queries in their place
+            }
             bool ok = !LAID || cross_wait(raw_full, 0, gone);
             if (ok && halves && elect_one()) {              // the queries' rotation: their own type against ones, into S's place
                 const uint32_t q_idesc = idesc | (p.f.q_dtype == TQ_BF16 ? 1u << 7 | 1u << 10 : 0u);
@@ -981,11 +994,16 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         const int i = warp >> 2, r = tid & 127, row = row0 + (solo ? 0 : i * kCrossTile) + r;
         const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tm_s = tmem + 128 * i + lane_at, tm_o = tmem + 256 + 128 * i + lane_at;
+        const uint32_t tm_s = 128 * i + lane_at, tm_o = 256 + 128 * i + lane_at;      // tensor memory is allocated whole: it begins at zero
         bool ok = true;
         // ---- the queries: rotated, by a power of two to [512, 1024), into the images.  One tile: half of a row's columns each group --------------
         float q_scale = 0.0f;
         if (n > 0) {
+            if constexpr (!LAID) {
+                load_queries(256);
+                asm volatile("bar.sync 3, 288;" ::: "memory");      // and tensor memory is there
+                tc_fence_after();
+            }
             const uint32_t image = M::kQ + (solo ? 0 : i) * kCrossImage;
             auto take = [&](float top) {              // the largest of the row: what its numbers are multiplied by
                 const int by = cross_exponent(top * p.f.scale, 9);
@@ -1287,7 +1305,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 float v[32];
                 __syncwarp();
                 if (n > 0) {
-                    cross_ld(tmem + 256 + 128 * mine + lane_at + 32 * c, v);
+                    cross_ld(256 + 128 * mine + lane_at + 32 * c, v);
                     cross_ld_wait(v);
                 }
 #pragma unroll
@@ -1321,7 +1339,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
     __syncthreads();
     if (warp == 9) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512));
     }
 }
 
