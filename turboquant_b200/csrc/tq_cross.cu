@@ -19,18 +19,19 @@
 // come (43 us looked up, 53 laid out ahead, with 32 queries).
 //
 // S, then P, and O of two tiles are all of tensor memory: 2 x (128 + 128) columns.  With two tiles of query rows each warpgroup has one, and while it works out
-// exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn, and at
-// the end each brings its O to the larger of their maxima and the product that rotates back adds them.  The running maximum is raised only when a logit exceeds it by 2^8, which makes rescaling O rare; a row needs no other
-// thread but its own.  Where few rows have long sequences the tokens are cut over several blocks as well, whose rows a second kernel joins.
+// exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn; at the end each brings its O to the
+// larger of their maxima, and the product that rotates back adds them.  The running maximum is raised only when a logit exceeds it by 2^8, which makes
+// rescaling O rare; a row needs no other thread but its own.  Where few rows have long sequences the tokens are cut over several blocks as well: every group
+// leaves a partial, and a second kernel joins them.
 //
 // The rotations are matrix products too, with a matrix of ones and minus ones, exact in any type: the queries go through the tensor core as they come before the
 // first tile, and O, as two fp16 parts, behind the last, which also brings its columns into order.  As butterflies over registers they took as long as ten tiles: code that a
-// block runs once is fetched anew by every block, and that is what it costs.  (4 x 2048 queries on 4096 tokens: 645 us with butterflies in front, 568 so.)
+// block runs once is fetched anew by every block, and that is what it costs.  (4 x 2048 queries on 4096 tokens: 645 us with butterflies in front, 573 so.)
 //
 // What bounds it.  Many rows: products and exponentials follow each other through S and P of a tile, and two tiles in flight, all that tensor memory holds, keep
-// the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 565 us, 973 TFLOP/s.  Few
-// rows, long sequences: the same chain for one tile, 2 x 16 queries on 65536 tokens, 64 heads on 8, 176 us, 793 GB/s of codes.  Short ones: what a block does
-// before its first tile and behind its last, 11 and 9 of 30 thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 21 us.
+// the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 556 us, 989 TFLOP/s.  Few
+// rows, long sequences: the same chain for one tile, 2 x 16 queries on 65536 tokens, 64 heads on 8, 176 us, 792 GB/s of codes.  Short ones: what a block does
+// before its first tile and behind its last, some 20 thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 20.9 us, two tiles a block.
 //
 // Numbers are fp16 in the tensor core with fp32 sums, brought into fp16's range by powers of two: a query row by its largest element, the norms of
 // K and V by the largest of the tile.
@@ -528,10 +529,8 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             told[0] = found; told[1] = s.b; told[2] = s.local; told[3] = s.len; told[4] = s.qlen;
         }
         __syncthreads();
-        if (warp >= 12) {
-            found = told[0] != 0;
-            s.b = told[1]; s.local = told[2]; s.len = told[3]; s.qlen = told[4];
-        }
+        found = told[0] != 0;
+        s.b = told[1]; s.local = told[2]; s.len = told[3]; s.qlen = told[4];
         if (!found) return;                           // uniform over the block
     }
     const int rows = s.qlen * G, row0 = s.local * kTiles * kCrossTile;
