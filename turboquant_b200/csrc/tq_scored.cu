@@ -16,7 +16,7 @@
 // one head of a page range, every warp whole pages of its own.
 //
 // What bounds it: the look-ups.  A code byte of K is looked up twice and one of V once, and with the page loads that fills shared memory's pipe to 74 percent while
-// 63 percent of the issue slots are taken: 8 sequences of 32768 tokens, 32 heads on 8, 115 us, of which the decode 95 (342 MB, 3.6 TB/s) and the
+// 63 percent of the issue slots are taken: 8 sequences of 32768 tokens, 32 heads on 8, 113 us, of which the decode 95 (342 MB, 3.6 TB/s) and the
 // join 18; a second walk over K in the join's place would be as long as the decode.  Short sequences: the launches, 1024 tokens 10.4 us.
 #include <cmath>
 #include <cstring>
@@ -314,11 +314,12 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
             split_lds<8>(v_at + st + 9 * kScoredRow, v3);
             split_lds<16>(k_at + st, ka);
             split_lds<16>(k_at + st + 8 * kScoredRow, kb);
-            float hi_acc[NT][4], lo_acc[NT][4];
+            // Sums of both tables: apart with one tile, whose chain of products would be twice as long, together with two, for the registers.
+            float acc[2][4];
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) hi_acc[t][i] = lo_acc[t][i] = 0.0f;
+                for (int i = 0; i < 4; i++) acc[t][i] = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 uint32_t ra[4], rb[4], la[4], lb[4];
@@ -326,10 +327,11 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
                 scored_lookup(kb[w], lut_lane, rb, lb);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    mma16816(hi_acc[t], ra[0], rb[0], ra[1], rb[1], qf[t][4 * w], qf[t][4 * w + 1]);
-                    mma16816(lo_acc[t], la[0], lb[0], la[1], lb[1], qf[t][4 * w], qf[t][4 * w + 1]);
-                    mma16816(hi_acc[t], ra[2], rb[2], ra[3], rb[3], qf[t][4 * w + 2], qf[t][4 * w + 3]);
-                    mma16816(lo_acc[t], la[2], lb[2], la[3], lb[3], qf[t][4 * w + 2], qf[t][4 * w + 3]);
+                    float (&hi_acc)[4] = acc[t], (&lo_acc)[4] = acc[NT == 1 ? 1 : t];
+                    mma16816(hi_acc, ra[0], rb[0], ra[1], rb[1], qf[t][4 * w], qf[t][4 * w + 1]);
+                    mma16816(lo_acc, la[0], lb[0], la[1], lb[1], qf[t][4 * w], qf[t][4 * w + 1]);
+                    mma16816(hi_acc, ra[2], rb[2], ra[3], rb[3], qf[t][4 * w + 2], qf[t][4 * w + 3]);
+                    mma16816(lo_acc, la[2], lb[2], la[3], lb[3], qf[t][4 * w + 2], qf[t][4 * w + 3]);
                 }
             }
             float na = lds_half(kn_at + st), nb = lds_half(kn_at + st + 8 * kScoredRow);
@@ -344,8 +346,13 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
             float* const to = logits + (int64_t)(len - left) * G;
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                xa[t] = fmaf((hi_acc[t][0] + hi_acc[t][1]) + (lo_acc[t][0] + lo_acc[t][1]), na * k_scale[t], bias_a);
-                xb[t] = fmaf((hi_acc[t][2] + hi_acc[t][3]) + (lo_acc[t][2] + lo_acc[t][3]), nb * k_scale[t], bias_b);
+                float a = acc[t][0] + acc[t][1], b = acc[t][2] + acc[t][3];
+                if constexpr (NT == 1) {
+                    a += acc[1][0] + acc[1][1];
+                    b += acc[1][2] + acc[1][3];
+                }
+                xa[t] = fmaf(a, na * k_scale[t], bias_a);
+                xb[t] = fmaf(b, nb * k_scale[t], bias_b);
                 over |= fmaxf(xa[t], xb[t]) > m[t] + kRaiseThreshold;
                 if (4 * t + tg < G) {
                     if (ta < left) to[ta * G + 4 * t] = xa[t];
