@@ -29,9 +29,10 @@
 // block runs once is fetched anew by every block, and that is what it costs.  (4 x 2048 queries on 4096 tokens: 645 us with butterflies in front, 573 so.)
 //
 // What bounds it.  Many rows: products and exponentials follow each other through S and P of a tile, and two tiles in flight, all that tensor memory holds, keep
-// the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 556 us, 989 TFLOP/s.  Few
-// rows, long sequences: the same chain for one tile, 2 x 16 queries on 65536 tokens, 64 heads on 8, 176 us, 792 GB/s of codes.  Short ones: what a block does
-// before its first tile and behind its last, some 20 thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 20.9 us, two tiles a block.
+// the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 556 us, 989 TFLOP/s.  Few rows, long
+// sequences: the same chain for one tile, half of its exponentials' time the norms' loads and products (fp16 results), and V's look-ups: 2 x 16
+// queries on 65536 tokens, 64 heads on 8, 172 us, 810 GB/s of codes.  Short ones: what a block does before its first tile and behind its last, some 20
+// thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 20.7 us, two tiles a block.
 //
 // Numbers are fp16 in the tensor core with fp32 sums, brought into fp16's range by powers of two: a query row by its largest element, the norms of
 // K and V by the largest of the tile.
@@ -1095,8 +1096,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                    v[2 * e] *= f.x;
-                    v[2 * e + 1] *= f.y;
+                    up(mul2(pk(v[2 * e], v[2 * e + 1]), pk(f.x, f.y)), v[2 * e], v[2 * e + 1]);
                 }
             };
             // exp2 of 16 columns into fp16 pairs, and their sum
