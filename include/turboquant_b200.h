@@ -386,7 +386,8 @@ int tq_nc_write_dropped(int32_t* count);
  * sequence without tokens gives zeros (LSE -inf); rows that belong to no sequence are left as they are.  A negative length, one
  * beyond the page table or beyond total_tokens counts as no tokens, a range of cu_seqlens_q that is none as no rows, and a page id outside [0, num_blocks) reads
  * page 0; all are counted (tq_state_fault_counts).  The workspace (tq_cross_workspace_bytes; 256-byte aligned, no initialising) holds
- * partial rows where sequences are cut, and where many query rows share them the cached tokens as 16-bit rows.  The reference attends fresh keys and values only (turboquant/vllm_backend_fused.py:336-369). */
+ * partial rows where sequences are cut, and where many query rows share them the cached tokens as 16-bit rows.  The reference attends fresh keys and
+ * values only (turboquant/vllm_backend_fused.py:336-369). */
 size_t tq_cross_workspace_bytes(int batch, int total_q, int64_t total_tokens, int num_q_heads, int num_kv_heads, int max_pages, int out_dtype);
 int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* cu_seqlens_q, int batch, int num_q_heads, int num_kv_heads, int head_dim,
              const void* kv_cache, int64_t num_blocks, int block_size, int slot_bytes, const int32_t* page_table, int max_pages,
@@ -416,7 +417,7 @@ int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q_heads, int
  * Eviction by accumulated attention weight.  Of every sequence's len tokens, for each KV head, the last
  * `recent` stay and of the others those of the largest scores, min(len, keep) in all; a tie goes to the lower
  * position, a NaN counts as -inf.  What stays keeps its order and moves to positions 0, 1, ... : whole slots of K and V, in the pages of
- * out_page_table, or (null) in the sequence's own pages.
+ * out_page_table, or (null) in the sequence's own pages, which no other sequence may then share.
  *   page_table    int32 [batch][max_pages], seq_lens int32 [batch] (device)
  *   scores        fp32, element [b * batch stride + h * head stride + position]; max_tokens: positions a row has
  *   out_page_table int32 [batch][out_max_pages], at least min(keep, longest) tokens wide; its pages are none of those that the call reads
