@@ -360,11 +360,6 @@ __device__ __forceinline__ uint32_t cross_table(uint32_t at) {
     asm("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
     return v;
 }
-__device__ __forceinline__ float4 cross_lds_f4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
-    return v;
-}
 __device__ __forceinline__ float2 cross_lds_f2(uint32_t at) {
     float2 v;
     asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
