@@ -29,9 +29,9 @@
 // block runs once is fetched anew by every block, and that is what it costs.  (4 x 2048 queries on 4096 tokens: 645 us with butterflies in front, 573 so.)
 //
 // What bounds it.  Many rows: products and exponentials follow each other through S and P of a tile, and two tiles in flight, all that tensor memory holds, keep
-// the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 556 us, 989 TFLOP/s.  Few rows, long
+// the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 560 us, 980 TFLOP/s.  Few rows, long
 // sequences: the same chain for one tile, half of its exponentials' time the norms' loads and products (fp16 results), and V's look-ups: 2 x 16
-// queries on 65536 tokens, 64 heads on 8, 172 us, 810 GB/s of codes.  Short ones: what a block does before its first tile and behind its last, some 20
+// queries on 65536 tokens, 64 heads on 8, 173 us, 805 GB/s of codes.  Short ones: what a block does before its first tile and behind its last, some 20
 // thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 20.7 us, two tiles a block.
 //
 // Numbers are fp16 in the tensor core with fp32 sums, brought into fp16's range by powers of two: a query row by its largest element, the norms of
