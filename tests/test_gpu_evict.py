@@ -220,6 +220,46 @@ def test_lengths_and_pages_out_of_range_are_left_out_and_counted():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scores_in_place", [True, False])
+def test_pages_out_of_range_within_the_same_pages(scores_in_place):
+    """Rows of a source page that there is not stay out, and so do those of a page that there is not to move them to: their slots are as they were, whatever the
+    scratch held."""
+    cache, table, _, lens, scores = case([100, 90, 64, 3000], 3, 128, 40, 6)
+    lens[0] = 80                                   # (pages 5 and 6 of the table: not read)
+    table[0, 6] = -7
+    table[1, 3] = cache.shape[1]                   # a source page: positions 48 ... 63
+    table[2, 1] = -1                               # a source page that is a destination too: positions 16 ... 31
+    table[3, 100] = 10 ** 9
+    scores[1, :, 40:70] += 1                       # its rows are among those that stay
+    want, kept_want, old = cache.numpy().copy(), np.full((4, 3, 40), -1, np.int32), cache.numpy()
+    out_scores = scores.clone() if scores_in_place else torch.full((4, 3, 40), -7.0)
+    skipped = 0
+    for b in range(4):
+        for h in range(3):
+            kept = kept_of(scores[b, h].numpy(), int(lens[b]), 40, 5)
+            kept_want[b, h, :len(kept)] = kept
+            out_scores[b, h, :len(kept)] = scores[b, h, kept.tolist()]
+            for j, t in enumerate(kept):
+                from_page, to_page = int(table[b, t // PAGE]), int(table[b, j // PAGE])
+                if 0 <= from_page < cache.shape[1] and 0 <= to_page < cache.shape[1]:
+                    want[:, to_page, j % PAGE, h] = old[:, from_page, t % PAGE, h]
+                else:
+                    skipped += 1
+    assert skipped > 50
+    before = _cabi.state_fault_counts()[2]
+    d, d_scores = cache.to(DEV), scores.to(DEV)
+    d_out = None if scores_in_place else torch.full((4, 3, 40), -7.0, device=DEV)
+    pattern = torch.full((_cabi.lib().tq_evict_workspace_bytes(4, 3, 80, table.shape[1] * PAGE, 40, 1, int(scores_in_place)),), 0xA5, dtype=torch.uint8, device=DEV)
+    del pattern                                    # what the allocator gives next
+    kept, new_lens = TurboQuantPagedAttention(3, 128, 0.1, 3).evict(d, table.to(DEV), lens.to(DEV), d_scores, 40, 5, None, d_out)
+    np.testing.assert_array_equal(kept.cpu().numpy(), kept_want)
+    np.testing.assert_array_equal(new_lens.cpu().numpy(), np.minimum(lens.numpy(), 40))
+    np.testing.assert_array_equal(d.cpu().numpy(), want)
+    np.testing.assert_array_equal((d_scores if scores_in_place else d_out).cpu().numpy(), out_scores.numpy())
+    assert _cabi.state_fault_counts()[2] > before
+
+
+@pytest.mark.gpu
 def test_empty_batch():
     attn = TurboQuantPagedAttention(2, 128, 0.1, 2)
     kept, lens = attn.evict(torch.zeros(kv_cache_shape(1, PAGE, 2, 128), dtype=torch.uint8, device=DEV), torch.zeros(0, 1, dtype=torch.int32, device=DEV),

@@ -536,13 +536,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
             const int t = p.kept[((int64_t)b * H + h) * p.keep + j];
             int64_t at = -1;
             if (STAGE == 0 || t != j) {           // within the same pages a row that stays in its place is left alone
-                if (STAGE == 2) {
-                    at = 0;
-                } else {
-                    const int64_t from = in[t >> 4];
-                    if ((uint64_t)from < (uint64_t)p.num_blocks) at = from * p.half_bytes + ((int64_t)(t & 15) * H + h) * p.slot_bytes;
-                    else atomicAdd(&g_evict_faults, 1);
-                }
+                const int64_t from = in[t >> 4];
+                if ((uint64_t)from < (uint64_t)p.num_blocks) at = STAGE == 2 ? 0 : from * p.half_bytes + ((int64_t)(t & 15) * H + h) * p.slot_bytes;
+                else if (STAGE != 2) atomicAdd(&g_evict_faults, 1);      // (nothing was staged for it: it is left out on the way back too)
             }
             source[i] = at;
         }
