@@ -98,6 +98,35 @@ def test_the_table_itself_is_no_output_table(monkeypatch):
         _cabi.evict(**{**a, "out_page_table": a["page_table"]})
 
 
+@pytest.mark.parametrize("change, words", [
+    (dict(seq_lens=torch.tensor([64, -1], dtype=torch.int32)), "negative length"), (dict(seq_lens=torch.tensor([65, 1], dtype=torch.int32)), "needs 5 pages"),
+    (dict(page_table=torch.tensor([[0, 1, 2, 16], [0, 1, 2, 3]], dtype=torch.int32)), "page id out of range"),
+    (dict(out_page_table=torch.tensor([[0], [-1]], dtype=torch.int32)), "page id out of range"), (dict(scores=torch.zeros(2, 4, 63)), "room for 63"),
+])
+def test_what_the_debug_checks_find(monkeypatch, change, words):
+    monkeypatch.setattr(_cabi, "_cuda", lambda t, name: None)
+    monkeypatch.setenv("TQ_DEBUG_CHECKS", "1")
+    with pytest.raises(_cabi.TurboQuantError, match=words):
+        _cabi.evict(**{**_meta(seq_lens=torch.tensor([64, 17], dtype=torch.int32)), **change})
+
+
+@pytest.mark.gpu
+def test_debug_checks_of_the_public_call(monkeypatch):
+    """Found on the host ahead of any kernel; what is in order runs as ever."""
+    cache, table, out_table, lens, scores = case([64, 40], 2, 128, 20, 6)
+    attn = TurboQuantPagedAttention(2, 128, 0.1, 2)
+    bad = table.clone()
+    bad[1, 2] = cache.shape[1]
+    monkeypatch.setenv("TQ_DEBUG_CHECKS", "1")
+    d = cache.to(DEV)
+    for t, out in ((bad, out_table.to(DEV)), (bad, None)):
+        with pytest.raises(_cabi.TurboQuantError, match="page id out of range"):
+            attn.evict(d, t.to(DEV), lens.to(DEV), scores.to(DEV), 20, 0, out)
+    assert torch.equal(d.cpu(), cache)
+    check([64, 40], 2, 128, 20, 3)
+    check([64, 40], 2, 128, 20, 3, in_place=True, scores_in_place=True)
+
+
 def test_refusals_of_the_library():
     import ctypes
     L, one = _cabi.lib(), ctypes.c_void_p(4096)

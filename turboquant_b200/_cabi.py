@@ -681,6 +681,12 @@ def evict(kv_cache, page_table, seq_lens, scores, keep: int, recent: int, out_pa
         _paged(kv_cache, out_page_table, seq_lens)
         if B and out_page_table.data_ptr() == page_table.data_ptr():
             raise TurboQuantError("the output table is the page table itself: leave it out to evict within the same pages")
+    if debug_checks():
+        _check_pages(page_table, None, page_table.shape[1], seq_lens, nb, bs)
+        if B and int(seq_lens.max().item()) > scores.shape[2]:
+            raise TurboQuantError(f"a sequence has {int(seq_lens.max().item())} tokens but its scores have room for {scores.shape[2]}")
+        if out_page_table is not None:
+            _check_pages(out_page_table, None, out_page_table.shape[1], seq_lens.clamp(max=keep), nb, bs)
     if B == 0:
         return
     most = min(page_table.shape[1] * bs, scores.shape[2])

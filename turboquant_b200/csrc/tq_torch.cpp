@@ -369,7 +369,7 @@ PyObject* layer_scored(PyObject* o, PyObject* const* args, Py_ssize_t n) {
 PyObject* layer_evict(PyObject* o, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     Layer* self = reinterpret_cast<Layer*>(o);
-    if (n != 8) Py_RETURN_NONE;
+    if (n != 8 || debug_checks()) Py_RETURN_NONE;
     const at::Tensor *cache = cuda_tensor(args[0]), *table = cuda_tensor(args[1]), *lens = cuda_tensor(args[2]), *scores = cuda_tensor(args[3]);
     int64_t keep, recent;
     if (!byte_cache(cache) || !small_int(args[4], INT32_MAX, keep) || keep == 0 || !small_int(args[5], keep, recent)) Py_RETURN_NONE;
