@@ -423,7 +423,8 @@ int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q_heads, int
  *   out_page_table int32 [batch][out_max_pages], at least min(keep, longest) tokens wide; its pages are none of those that the call reads
  *   out_scores    fp32, the kept scores by their new position; may be `scores` itself
  *   kept          int32 [batch][num_kv_heads][keep]: the position each kept token had, ascending, then -1
- *   new_lens      int32 [batch]: min(len, keep)
+ *   new_lens      int32 [batch]: min(len, keep); may be `seq_lens` itself
+ * These two apart, out_scores on `scores` and new_lens on `seq_lens`, no output may overlap what the call reads, or another output.
  * Slots, scores and pages behind the last kept token are left as they are.  A sequence of a negative length, or longer than its
  * pages or scores, keeps nothing and is counted, as is a page id outside [0, num_blocks), whose rows are not moved (tq_state_fault_counts).
  * block_size 16; any slot of a multiple of 4 bytes.  The workspace (tq_evict_workspace_bytes, max_tokens = the smaller of 16 max_pages and the scores'

@@ -147,6 +147,27 @@ def test_refusals_of_the_library():
     assert f(2, 4, 80, 64, 16, 0, 0) == 0 and f(2, 4, 80, 64, 17, 1, 0) == 2 * 2 * 32 * 4 * 80 and f(2, 4, 80, 64, 17, 0, 1) == 768
 
 
+def test_outputs_that_overlap_what_is_read_are_refused():
+    """Blocks that read a length, a table or a score while another writes there would not agree.  (All calls are refused: the addresses are none.)"""
+    import ctypes
+    L, I, Q, base = _cabi.lib(), ctypes.c_int, ctypes.c_int64, 1 << 20
+    at = dict(cache=base, table=2 * base, lens=3 * base, scores=4 * base, out_table=5 * base, out=6 * base, kept=7 * base, new=8 * base)
+
+    def call(**change):
+        a = {k: ctypes.c_void_p(v) for k, v in {**at, **change}.items()}
+        rc = L.tq_evict(a["cache"], Q(16), I(16), I(4), I(80), a["table"], I(4), a["lens"], I(2), a["scores"], Q(256), Q(64), I(64), I(16), I(0), a["out_table"], I(1),
+                        a["out"], Q(64), Q(16), a["kept"], a["new"], None, ctypes.c_size_t(0), None)
+        return rc, L.tq_last_error().decode()
+    for out, size in (("out", 4 * (64 + 3 * 16 + 16)), ("kept", 4 * 2 * 4 * 16), ("new", 8)):
+        for inp, length in (("table", 32), ("lens", 8), ("out_table", 8)):
+            for shift in (4 - size, length - 4):
+                rc, words = call(**{out: at[inp] + shift})
+                assert rc == 1 and "overlaps the lengths or a table" in words, (out, inp, shift)
+    for change in (dict(kept=at["scores"] + 4 * 511), dict(kept=at["out"] - 4 * 127), dict(new=at["kept"] + 4 * 127), dict(new=at["scores"] - 4), dict(new=at["out"] + 4 * 127)):
+        rc, words = call(**change)
+        assert rc == 1 and "kept or new_lens overlaps" in words, change
+
+
 # ---- on the GPU ------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens, keep, recent", [
@@ -326,3 +347,18 @@ def test_captured_beside_another_graph_and_on_another_stream():
             np.testing.assert_array_equal(new.cpu().numpy(), want[1])
             np.testing.assert_array_equal(d[0].cpu().numpy(), want[2])
             np.testing.assert_array_equal(d[3].cpu().numpy(), want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("lens, heads, keep", [([100, 0, 500, 37] * 8, 8, 40), ([30000, 5, 9000], 8, 1000), ([70000], 4, 65000), ([2000] * 40, 16, 1999)])
+def test_the_new_lengths_may_replace_the_old_ones(lens, heads, keep, in_place):
+    """`new_lens` is `seq_lens`: every head of a sequence sees the old length, in blocks that start late too."""
+    cache, table, out_table, lens_t, scores = case(lens, heads, 64, keep, 3)
+    out_table = table if in_place else out_table
+    want = expected(cache, table, out_table, lens_t, scores, torch.zeros(len(lens), heads, keep), keep, 7)
+    d_cache, d_lens, out = cache.to(DEV), lens_t.to(DEV), torch.zeros(len(lens), heads, keep, device=DEV)
+    kept = torch.empty(len(lens), heads, keep, dtype=torch.int32, device=DEV)
+    _cabi.evict(d_cache, table.to(DEV), d_lens, scores.to(DEV), keep, 7, None if in_place else out_table.to(DEV), out, kept, d_lens)
+    for got, w in ((kept, want[0]), (d_lens, want[1]), (d_cache, want[2]), (out, want[3])):
+        np.testing.assert_array_equal(got.cpu().numpy(), w)

@@ -129,10 +129,7 @@ __global__ void __launch_bounds__(KEPT ? kEvictThreads : kEvictManyThreads, KEPT
     bool bad;
     const int len = evict_len(p, b, bad);
     const int n = min(len, p.keep), recent = min(p.recent, n), M = len - recent, k = n - recent;
-    if (h == 0 && rank == 0 && tid == 0) {
-        p.new_lens[b] = n;
-        if (bad) atomicAdd(&g_evict_faults, 1);
-    }
+    if (bad && h == 0 && rank == 0 && tid == 0) atomicAdd(&g_evict_faults, 1);
     const float* const row = p.scores + b * p.score_b + h * p.score_h;
     float* const to = p.score_to + b * p.to_b + h * p.to_h;
     int32_t* const kept = p.kept + (int64_t)unit * p.keep;
@@ -510,6 +507,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     const int b = blockIdx.x / p.out_pages, page = blockIdx.x - b * p.out_pages;
     bool bad;
     const int n = min(evict_len(p, b, bad), p.keep), tokens = min(16, n - 16 * page);
+    // The new lengths may replace the old ones: they are written behind the selection, whose blocks all have to see the same length, and a block of this
+    // launch that reads one already replaced comes to the same n.
+    if (STAGE != 1 && page == 0 && threadIdx.x == 0) p.new_lens[b] = n;
     if (tokens <= 0) return;
     if (STAGE != 1 && p.scores_staged) {          // the kept scores of this page's positions back to where they came from
         for (int i = threadIdx.x; i < p.kv_heads * 16; i += kMoveThreads) {
@@ -671,6 +671,19 @@ extern "C" int tq_evict(void* kv_cache, int64_t num_blocks, int block_size, int 
                                scores < out_scores + last(out_batch_stride, out_head_stride, longest);
     const size_t need = tq_evict_workspace_bytes(batch, num_kv_heads, slot_bytes, most, keep, in_place, scores_staged);
     TQ_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), TQ_ERR_WORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, need);
+    // Blocks read lengths, tables and scores while others write: what is written may be `scores` and, word for word, `seq_lens`, nothing else that is read.
+    struct Span { const void* at; int64_t words; };
+    auto meet = [](Span a, Span b) {
+        return a.at && b.at && (uintptr_t)a.at < (uintptr_t)b.at + 4 * (uint64_t)b.words && (uintptr_t)b.at < (uintptr_t)a.at + 4 * (uint64_t)a.words;
+    };
+    const Span s_lens{seq_lens, batch}, s_table{page_table, (int64_t)batch * max_pages}, s_out_table{out_page_table, (int64_t)batch * out_max_pages},
+        s_scores{scores, last(score_batch_stride, score_head_stride, most)}, s_out{out_scores, last(out_batch_stride, out_head_stride, longest)},
+        s_kept{kept, (int64_t)batch * num_kv_heads * keep}, s_new{new_lens, batch};
+    for (const Span& w : {s_out, s_kept, s_new})
+        TQ_REQUIRE(!meet(w, s_table) && !meet(w, s_out_table) && (!meet(w, s_lens) || w.at == new_lens && new_lens == seq_lens), TQ_ERR_INVALID,
+                   "an output overlaps the lengths or a table");
+    TQ_REQUIRE(!meet(s_kept, s_scores) && !meet(s_kept, s_out) && !meet(s_kept, s_new) && !meet(s_new, s_scores) && !meet(s_new, s_out), TQ_ERR_INVALID,
+               "kept or new_lens overlaps scores, or one the other");
     TQ_REQUIRE((int64_t)batch * num_kv_heads < 1 << 26 && (int64_t)batch * out_pages < 1ll << 31, TQ_ERR_UNSUPPORTED, "too many rows for one launch");
 
     EvictParams p{};
