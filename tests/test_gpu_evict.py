@@ -362,3 +362,14 @@ def test_the_new_lengths_may_replace_the_old_ones(lens, heads, keep, in_place):
     _cabi.evict(d_cache, table.to(DEV), d_lens, scores.to(DEV), keep, 7, None if in_place else out_table.to(DEV), out, kept, d_lens)
     for got, w in ((kept, want[0]), (d_lens, want[1]), (d_cache, want[2]), (out, want[3])):
         np.testing.assert_array_equal(got.cpu().numpy(), w)
+
+
+@pytest.mark.gpu
+def test_the_largest_keep():
+    """A budget of 2^31 - 1 tokens (every token stays): the places behind the sequence are filled to the last."""
+    keep = 2 ** 31 - 1
+    cache, table, _, lens, scores = case([100], 1, 64, 128, 3)
+    d = cache.to(DEV)
+    kept, new_lens = TurboQuantPagedAttention(1, 64, 0.1, 1).evict(d, table.to(DEV), lens.to(DEV), scores.to(DEV), keep, 0, None, torch.zeros(1, 1, 112, device=DEV))
+    assert new_lens.tolist() == [100] and torch.equal(d.cpu(), cache) and kept.shape == (1, 1, keep)
+    assert kept[0, 0, :100].tolist() == list(range(100)) and int(kept[0, 0, 100:].amin()) == int(kept[0, 0, 100:].amax()) == -1

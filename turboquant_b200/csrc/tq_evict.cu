@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(KEPT ? kEvictThreads : kEvictManyThreads, KEPT
         kept[k + j] = M + j;
         to[k + j] = row[M + j];
     }
-    for (int j = n + me; j < p.keep; j += all) kept[j] = -1;
+    for (int64_t j = n + me; j < p.keep; j += all) kept[j] = -1;      // (keep may be the largest int)
     if (k == M) {                      // all of them (uniform over the cluster, as the way out below is)
         for (int j = me; j < k; j += all) {
             kept[j] = j;
