@@ -168,6 +168,16 @@ def test_outputs_that_overlap_what_is_read_are_refused():
         assert rc == 1 and "kept or new_lens overlaps" in words, change
 
 
+@pytest.mark.parametrize("batch_stride, head_stride", [(16, 16), (63, 16), (48, 17), (16, 31), (32, 32)])
+def test_rows_of_kept_scores_that_meet_across_heads_and_sequences_are_refused(batch_stride, head_stride):
+    """Two sequences of four heads, 16 scores each: every stride holds a row, but rows of one sequence lie on another's."""
+    import ctypes
+    L, I, Q, one = _cabi.lib(), ctypes.c_int, ctypes.c_int64, ctypes.c_void_p(4096)
+    rc = L.tq_evict(one, Q(16), I(16), I(4), I(80), one, I(4), one, I(2), one, Q(256), Q(64), I(64), I(16), I(0), one, I(1), ctypes.c_void_p(1 << 20), Q(batch_stride),
+                    Q(head_stride), one, one, None, ctypes.c_size_t(0), None)
+    assert rc == 1 and "rows of out_scores overlap" in L.tq_last_error().decode()
+
+
 # ---- on the GPU ------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens, keep, recent", [

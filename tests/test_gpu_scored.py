@@ -95,6 +95,16 @@ def test_refusals_of_the_library():
     assert call(cache=ctypes.c_void_p(4100))[0] == 1 and "overlap" in call(sh=31)[1]
 
 
+@pytest.mark.parametrize("batch_stride, head_stride", [(32, 32), (127, 32), (32, 63), (100, 40)])
+def test_rows_of_scores_that_meet_across_heads_and_sequences_are_refused(batch_stride, head_stride):
+    """Two sequences of four heads, 32 scores each: every stride holds a row, but rows of one sequence lie on another's."""
+    import ctypes
+    L, P, I, Q = _cabi.lib(), ctypes.c_void_p(4096), ctypes.c_int, ctypes.c_int64
+    rc = L.tq_decode_scored(P, I(1), I(2), I(8), I(4), I(128), P, Q(4), I(16), I(80), P, I(2), P, P, ctypes.c_float(0.1), P, Q(batch_stride), Q(head_stride), I(32), I(1),
+                            P, ctypes.c_size_t(0), P, I(1), None, None)
+    assert rc == 1 and "rows of scores overlap" in L.tq_last_error().decode()
+
+
 # ---- on the GPU -----------------------------------------------------------------------------------
 GEOMETRIES = [(8, 2, 128), (5, 1, 128), (16, 2, 128), (3, 3, 96), (21, 3, 128), (12, 4, 96), (24, 8, 65)]
 
@@ -249,3 +259,13 @@ def test_graphs_and_streams():
         assert torch.equal(e, runs[0][3]) and torch.equal(eager, runs[0][4])
         for _, scores, out, want, want_s, *_ in runs:
             assert torch.equal(out, want) and torch.equal(scores, want_s)
+
+
+@pytest.mark.gpu
+def test_scores_of_heads_ahead_of_sequences():
+    """Scores kept [head][sequence][token]: rows that do not meet are taken in any order."""
+    _, inputs, out, scores, lse = run([500, 40, 0], 6, 3)
+    cache, table, lens, q, before = inputs
+    turned = before.permute(1, 0, 2).contiguous().to(DEV)
+    got = TurboQuantPagedAttention(6, 128, 1 / math.sqrt(128), 3).decode_scored(q.to(DEV), cache.to(DEV), table.to(DEV), lens.to(DEV), turned.permute(1, 0, 2))
+    assert torch.equal(got.cpu(), out) and np.array_equal(turned.permute(1, 0, 2).cpu().numpy(), scores)

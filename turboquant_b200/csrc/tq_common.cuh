@@ -32,6 +32,15 @@ int fail(int code, const char* fmt, ...);
             return ::tq::fail(TQ_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e__)); \
     } while (0)
 
+// Whether rows of n elements at b * sb + h * sh (strides not negative) can meet: the smaller stride has to hold a row, the larger all rows along the smaller.
+inline bool rows_overlap(int64_t batch, int64_t heads, int64_t sb, int64_t sh, int64_t n) {
+    if (n <= 0 || (batch <= 1 && heads <= 1)) return false;
+    if (batch <= 1) return sh < n;
+    if (heads <= 1) return sb < n;
+    const int64_t small = sb < sh ? sb : sh, large = sb < sh ? sh : sb, along = (sb < sh ? batch : heads) - 1;
+    return small < n || (large - n) / along < small;
+}
+
 // Codebook constants shared by every translation unit (defined in tq_api.cu).
 void host_codebook(int dim, int bits, float* centroids, float* boundaries);
 extern const double kCentroidsN01_4bit[16];

@@ -662,8 +662,7 @@ extern "C" int tq_evict(void* kv_cache, int64_t num_blocks, int block_size, int 
                longest, out_pages);
     TQ_REQUIRE(most <= 1 << 30, TQ_ERR_UNSUPPORTED, "sequences of more than 2^30 tokens");
     TQ_REQUIRE(score_batch_stride >= 0 && score_head_stride >= 0 && out_batch_stride >= 0 && out_head_stride >= 0, TQ_ERR_INVALID, "negative stride");
-    TQ_REQUIRE((batch == 1 || out_batch_stride >= longest) && (num_kv_heads == 1 || out_head_stride >= longest), TQ_ERR_INVALID,
-               "the rows of out_scores overlap");
+    TQ_REQUIRE(!rows_overlap(batch, num_kv_heads, out_batch_stride, out_head_stride, longest), TQ_ERR_INVALID, "the rows of out_scores overlap");
     // Scores that are written where scores are read wait until all have been read.
     auto last = [&](int64_t sb, int64_t sh, int64_t n) { return (batch - 1) * sb + (num_kv_heads - 1) * sh + n; };
     const bool in_place = out_page_table == nullptr;

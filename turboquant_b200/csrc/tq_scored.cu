@@ -689,7 +689,7 @@ extern "C" int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q
     TQ_REQUIRE(max_pages >= 1 && max_pages <= 1 << 26 && score_tokens >= 0 && new_tokens >= 0, TQ_ERR_INVALID, "bad size");
     TQ_REQUIRE(score_batch_stride >= 0 && score_head_stride >= 0, TQ_ERR_INVALID, "negative stride");
     const int64_t most = (int64_t)max_pages * kPageTokens < score_tokens ? (int64_t)max_pages * kPageTokens : score_tokens;
-    TQ_REQUIRE((batch == 1 || score_batch_stride >= most) && (num_kv_heads == 1 || score_head_stride >= most), TQ_ERR_INVALID, "the rows of scores overlap");
+    TQ_REQUIRE(!rows_overlap(batch, num_kv_heads, score_batch_stride, score_head_stride, most), TQ_ERR_INVALID, "the rows of scores overlap");
     TQ_REQUIRE(((uintptr_t)kv_cache & 15) == 0 && ((uintptr_t)workspace & 255) == 0, TQ_ERR_INVALID, "kv_cache must be 16-byte aligned, the workspace 256-byte");
     TQ_REQUIRE((int64_t)batch * num_q_heads < 1 << 24, TQ_ERR_UNSUPPORTED, "too many rows for one launch");
     int sms = 0;
