@@ -404,9 +404,12 @@ int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* cu_seqlens_
  * head_dim 65 ... 128 (80-byte slots), any number of KV heads, up to 8 query heads on each.  Logits are worked out to about 2^-20, so that scores are fp32
  * sums in earnest; out is as exact as its 16-bit types.  Results do not depend on an order of atomics.  Scores behind a sequence are left as they are.  A
  * sequence longer than its page table, or of a negative length, has output zero and no weights; one longer than its scores has its output and
- * leaves its scores alone; both are counted, and so is a page id outside [0, num_blocks), for which page 0 is read (tq_state_fault_counts).
+ * leaves its scores alone; both are counted, and so is a page id outside [0, num_blocks), for which page 0 is read (tq_state_fault_counts).  A page whose
+ * copy does not come within the (bounded) wait for it is counted too: the KV heads that it belongs to have outputs of NaN with an LSE of +inf, and their scores are
+ * left as they are.  tq_scored_lose_copies(1), for tests: the calls this process makes afterwards bring in no page; 0: as ever.
  * The workspace (tq_decode_scored_workspace_bytes; 256-byte aligned, no initialising) holds a logit for every query head and slot of the page table.
  * No counterpart in the reference. */
+int tq_scored_lose_copies(int on);
 size_t tq_decode_scored_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_pages);
 int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q_heads, int num_kv_heads, int head_dim, const void* kv_cache,
                      int64_t num_blocks, int block_size, int slot_bytes, const int32_t* page_table, int max_pages, const int32_t* seq_lens,

@@ -269,3 +269,27 @@ def test_scores_of_heads_ahead_of_sequences():
     turned = before.permute(1, 0, 2).contiguous().to(DEV)
     got = TurboQuantPagedAttention(6, 128, 1 / math.sqrt(128), 3).decode_scored(q.to(DEV), cache.to(DEV), table.to(DEV), lens.to(DEV), turned.permute(1, 0, 2))
     assert torch.equal(got.cpu(), out) and np.array_equal(turned.permute(1, 0, 2).cpu().numpy(), scores)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens, Hq, H", [([300, 0, 17], 8, 2), ([20000], 8, 2), ([9000, 3], 10, 2), ([40, 700] * 50, 4, 4)])
+def test_pages_that_never_come_leave_the_scores_alone(lens, Hq, H):
+    """As after waits that ran out: rows are void, and none of the logits, worked out from whatever lay there, reaches a score, whether a head is whole, cut, or
+    one of many sequences.  The next call is as ever."""
+    cache, table, lens_t = paged(lens, H, 128, 4)
+    q = torch.randn(len(lens), Hq, 128, generator=torch.Generator().manual_seed(0)).half()
+    attn = TurboQuantPagedAttention(Hq, 128, 0.1, H)
+    before = torch.rand(len(lens), H, table.shape[1] * PAGE)
+    scores, lse, d = before.to(DEV), torch.zeros(len(lens), Hq, device=DEV), [t.to(DEV) for t in (q, cache, table, lens_t)]
+    _cabi.scored_lose_copies(True)
+    try:
+        out = attn.decode_scored(*d, scores, None, lse).cpu()
+        torch.cuda.synchronize()
+    finally:
+        _cabi.scored_lose_copies(False)
+    assert torch.equal(scores.cpu(), before)
+    some = lens_t > 0
+    assert out[some].isnan().all() and (lse.cpu()[some] == np.inf).all()
+    assert not out[~some].any() and (lse.cpu()[~some] == -np.inf).all()
+    out = attn.decode_scored(*d, scores, None, lse).cpu()
+    check((cache, table, lens_t, q, before), out, scores.cpu().numpy(), lse.cpu().numpy(), scale=0.1)

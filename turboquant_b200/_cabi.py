@@ -35,7 +35,7 @@ EXPORTS = (
     "tq_dequant_paged", "tq_pages_packed_bytes", "tq_pages_gather", "tq_pages_scatter",
     "tq_decode_max_query_columns", "tq_set_exchange_wait_limit", "tq_decode_static_status", "tq_fault_counts",
     "tq_write_guard_stats", "tq_pages_packed_bytes_for_slot", "tq_cross_workspace_bytes", "tq_cross",
-    "tq_decode_scored_workspace_bytes", "tq_decode_scored", "tq_evict_workspace_bytes",
+    "tq_scored_lose_copies", "tq_decode_scored_workspace_bytes", "tq_decode_scored", "tq_evict_workspace_bytes",
     "tq_evict", "tq_state_fault_counts",
 )
 
@@ -554,6 +554,11 @@ def state_fault_counts():
     c = (ctypes.c_int32 * 3)()
     _check(lib().tq_state_fault_counts(c))
     return tuple(int(x) for x in c)
+
+
+def scored_lose_copies(on: bool) -> None:
+    """For tests: ``decode_scored`` acts from here on as if no page came in."""
+    _check(lib().tq_scored_lose_copies(ctypes.c_int(on)))
 
 
 def _same_device(t: torch.Tensor, others) -> None:

@@ -44,10 +44,15 @@ struct ScoredParams {
     int64_t score_b, score_h;
     int64_t room;              // tokens of a row of logits
     int score_room, new_tokens, chunks;
+    int lose;                  // tests: no copy comes
     uint16_t rest_h[16];       // second table
 };
 
 static __device__ int32_t g_scored_faults = 0;
+static int g_scored_lose = 0;
+// The running maximum that a warp leaves behind a copy that never came, with a sum of +inf: the rows' lse is +inf then, which no logits add up to
+// (one of +inf gives NaN), and tells the join.
+constexpr float kScoredVoid = 3.0e38f;
 
 // The slots of a page in one tensor copy, as in the split decode, but first to leave L2: read once, while the logits written meanwhile are read again.
 __device__ __forceinline__ void scored_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t policy) {
@@ -78,7 +83,7 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
     const int g = lane >> 2, tg = lane & 3;
     const uint32_t smem_base = smem_u32(smem);
     const int G = p.group;
-    if (smem_base + kScoredBelow * kScoredRing > kLutAddr) {   // the map does not fit: nothing is computed, the join finds no plan
+    if (smem_base + kScoredBelow * kScoredRing > kLutAddr) {   // the map does not fit: nothing is computed, the join finds a list without work
         grid_dependency_wait();
         if (tid == 0 && blockIdx.x == 0) {
             p.header[1] = 0;
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
     const uint32_t v_at = split_keep(ring_at + kScoredHalf + 2 * tg * kScoredRow + g * 8), vn_at = kn_at + kScoredHalf;
     const uint32_t full_at = split_keep(smem_u32(&full_s[warp][0]));
     uint32_t stage = 0, parity = 0;
-    bool lost = false, bad_page = false;
+    bool lost = sp.lose != 0, bad_page = false;
 
     while (pos < hi) {
         // ---- the next segment: a page range of one head -------------------------------------------------
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
                 bool there = false;
                 for (uint32_t i = 0; i < kSpinLimit && !there; i++) there = split_try_wait(full_at + 8 * stage, parity);
                 if (!__all_sync(0xffffffffu, there)) {
-                    lost = true;      // the output is void; what is still in flight gets its time to land
+                    lost = true;      // the heads from here on are void; what is still in flight gets its time to land
                     if (lane == 0) atomicAdd(&g_scored_faults, 1);
                     for (uint32_t k = 1; k < kScoredStages; k++) {
                         const bool wraps = stage + k >= kScoredStages;
@@ -425,6 +430,14 @@ __global__ void __launch_bounds__(kScoredThreads, 1) decode_scored_kernel(const 
         }
 
         // ---- combine the group's warps ------------------------------------------------------------------------
+        if (lost) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                m[t] = kScoredVoid;
+                l[t] = INFINITY;
+            }
+            v_scale = NAN;
+        }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -530,7 +543,8 @@ __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_
             count = (int)((end * s.workers + s.total - 1) / s.total) - first;
         }
     }
-    const bool fits = given <= sp.score_room && np == (given > 0 ? (given + kPageTokens - 1) / kPageTokens : 0) && given >= 0;
+    // (a list without work although there are tokens: nothing was computed)
+    const bool fits = given <= sp.score_room && (given <= 0 || s.total > 0) && np == (given > 0 ? (given + kPageTokens - 1) / kPageTokens : 0) && given >= 0;
     if (!fits && head == 0 && chunk == 0 && tid == 0) atomicAdd(&g_scored_faults, 1);
     // The first tokens' logits and scores are on their way while the lse is worked out.
     const int64_t step = (int64_t)sp.chunks * kJoinThreads, t_first = (int64_t)chunk * kJoinThreads + tid;
@@ -549,6 +563,7 @@ __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_
     };
     if (fits) fetch(t_first);
     auto slot_row = [&](int i, int r) -> int64_t { return ((int64_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * hs + hsub) * G + r; };
+    bool gone = false;
     for (int r = warp; r < G; r += kWarps) {
         float lse = -INFINITY;
         if (count == 1) {
@@ -562,11 +577,12 @@ __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_
             for (int i = lane; i < count; i += 32) sum += fast_exp2(p.partial_lse[slot_row(i, r)] - top);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            lse = sum == 0.0f ? -INFINITY : top + log2f(sum);
+            lse = sum == 0.0f ? -INFINITY : top == INFINITY ? top : top + log2f(sum);
         }
+        gone |= lse == INFINITY;
         if (lane == 0) lse_s[r] = lse;
     }
-    __syncthreads();
+    gone = __syncthreads_or(gone);
     if (count != 1) {
         for (int r = chunk; r < G; r += sp.chunks) {
             const float lse = lse_s[r];
@@ -592,7 +608,7 @@ __global__ void __launch_bounds__(kJoinThreads) scored_join_kernel(const __grid_
             __syncthreads();
         }
     }
-    if (!fits) return;
+    if (!fits || gone) return;          // (void rows have no weights: the scores, which outlast the call, stay as they are)
     float lse[8];
 #pragma unroll
     for (int r = 0; r < 8; r++) lse[r] = r < G && lse_s[r] != -INFINITY ? lse_s[r] : INFINITY;      // a row without a weight: exp2(x - inf) = 0
@@ -665,6 +681,11 @@ static int launch_scored_kernel(const ScoredParams& p, cudaStream_t s) {
 }
 
 }  // namespace tq
+
+extern "C" int tq_scored_lose_copies(int on) {
+    tq::g_scored_lose = on != 0;
+    return TQ_OK;
+}
 
 extern "C" size_t tq_decode_scored_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_pages) {
     int sms = 0;
@@ -747,6 +768,7 @@ extern "C" int tq_decode_scored(const void* q, int q_dtype, int batch, int num_q
     sp.room = (int64_t)max_pages * kPageTokens;
     sp.score_room = score_tokens;
     sp.new_tokens = new_tokens;
+    sp.lose = g_scored_lose;
     // A block of the join for every 256 tokens, up to eight an SM in all (and one a row at least).
     const int64_t runs = (most + kJoinThreads - 1) / kJoinThreads, fit = (int64_t)8 * sms / ((int64_t)batch * num_kv_heads);
     sp.chunks = (int)(runs < 1 ? 1 : runs < (fit > 1 ? fit : 1) ? runs : (fit > 1 ? fit : 1));
