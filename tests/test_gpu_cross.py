@@ -251,6 +251,27 @@ def test_repeats_exactly_and_reads_nothing_behind_a_sequence():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q_lens, lens", [([16], [200]), ([5, 7], [9000, 100]), ([100, 1, 0, 30], [1500, 300, 50, 0]), ([600], [2000]), ([200, 100], [300, 200])])
+def test_another_width_of_the_table_and_more_tokens_give_the_same_bits(q_lens, lens, dtype):
+    """Where a sequence's tokens are cut follows from its own length: neither from the table's width nor from the tokens that the caller makes room for."""
+    cache, table, lens_t = paged(lens, 2, 128, 4)
+    q = torch.randn(sum(q_lens), 4, 128, generator=torch.Generator().manual_seed(0)).to(dtype)
+    cu = torch.tensor([0, *np.cumsum(q_lens)], dtype=torch.int32)
+    attn = TurboQuantPagedAttention(4, 128, 0.1, 2)
+    wide = torch.full((len(lens), 5000), 10 ** 9, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    d_q, d_cu, d_cache, d_lens = q.to(DEV), cu.to(DEV), cache.to(DEV), lens_t.to(DEV)
+    results = []
+    for t, total in ((table, sum(lens)), (wide, sum(lens)), (table, 10 ** 5), (wide, 10 ** 5)):
+        lse = torch.full((q.shape[0], 4), 77.0, device=DEV)
+        results.append((attn.cross(d_q, d_cu, d_cache, t.to(DEV), d_lens, total, None, lse), lse))
+    for out, lse in results[1:]:
+        assert torch.equal(out, results[0][0]) and torch.equal(lse, results[0][1])
+    check((cache, table, lens_t, cu, q), results[3][0].cpu(), results[3][1].cpu().numpy(), scale=0.1)
+
+
+@pytest.mark.gpu
 def test_out_of_range_is_left_out_and_counted():
     cache, table, lens = paged([64, 64, 64, 64], 2, 128, 4)
     q = torch.randn(40, 4, 128, generator=torch.Generator().manual_seed(0)).half()

@@ -72,7 +72,7 @@ struct CrossParams {
     int64_t kv_room;            // tiles that there is room for
     float* partial_o;           // [cut][group][query row][query head][128], rotated domain
     float* partial_lse;
-    int total_q, splits;
+    int total_q, splits;        // of the tokens: most blocks that a sequence is cut over
     uint16_t level_h[16];
 };
 
@@ -82,6 +82,7 @@ struct CrossSeq {
     int b, local;               // the sequence, and which of its items the index is
     int len, qlen;              // tokens, query rows (tokens of the prompt)
     int kv0;                    // its first tile of tokens
+    int cuts;                   // blocks that its tokens are cut over
 };
 
 __device__ __forceinline__ int cross_len(const CrossParams& p, int b, bool& bad) {
@@ -94,6 +95,9 @@ __device__ __forceinline__ int cross_qlen(const CrossParams& p, int b, bool& bad
     bad = c0 < 0 || c1 < c0 || c1 > p.total_q;
     return bad ? 0 : c1 - c0;
 }
+// Blocks that a sequence's tokens are cut over: two tiles each (one a warpgroup) at least.  By its own length: results depend neither on the table's width nor on
+// the tokens that the caller makes room for, and no block beside these has work (or a partial).
+__device__ __forceinline__ int cross_cuts(const CrossParams& p, int len) { return max(1, min(p.splits, (len + 2 * kCrossTile - 1) / (2 * kCrossTile))); }
 __device__ __forceinline__ int cross_upto(int v, int lane) {      // the sum of the lanes up to this one
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -139,6 +143,7 @@ __device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, 
             const int64_t kv_to = kv + cross_upto(kt, lane);
             s.b += l;
             s.local = (int)(index - items) - __shfl_sync(0xffffffffu, to - mine, l);
+            if constexpr (KIND != 0) s.cuts = __shfl_sync(0xffffffffu, cross_cuts(p, s.len), l);
             s.len = __shfl_sync(0xffffffffu, kv_to <= p.kv_room ? s.len : 0, l);
             s.qlen = __shfl_sync(0xffffffffu, s.qlen, l);
             s.kv0 = (int)__shfl_sync(0xffffffffu, kv_to - kt, l);
@@ -515,24 +520,28 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
     CrossSeq s;
     const int64_t item = blockIdx.x / p.splits;
     const int split = (int)(blockIdx.x - item * p.splits), h = (int)(item % H);
+    volatile int* const told = reinterpret_cast<volatile int*>(window + M::kBars + 416);
+    auto cut_over = [&] { return (int)lds32(M::kBars + 416 + 20); };      // read again where it is needed: a register less
     if constexpr (LAID) {
         if (!cross_find<kTiles>(p, item / H, lane, s)) return;            // uniform over the block
+        if (tid == 0) told[5] = s.cuts;
     } else {
-        int* const told = reinterpret_cast<int*>(window + M::kBars + 416);
         bool found = true;
         if (warp < 12) found = cross_find<kTiles>(p, item / H, lane, s);
         if (tid == 0) {
-            told[0] = found; told[1] = s.b; told[2] = s.local; told[3] = s.len; told[4] = s.qlen;
+            told[0] = found; told[1] = s.b; told[2] = s.local; told[3] = s.len; told[4] = s.qlen; told[5] = s.cuts;
         }
         __syncthreads();
         found = told[0] != 0;
-        s.b = told[1]; s.local = told[2]; s.len = told[3]; s.qlen = told[4];
+        s.b = told[1]; s.local = told[2]; s.len = told[3]; s.qlen = told[4]; s.cuts = told[5];
         if (!found) return;                           // uniform over the block
     }
+    if (split >= s.cuts) return;                      // so is this (as one condition with the search's it costs the laid-out form 200 bytes of spills)
     const int rows = s.qlen * G, row0 = s.local * kTiles * kCrossTile;
     const bool solo = kTiles == 1 || rows - row0 <= kCrossTile;           // one tile of query rows
     const int all = (s.len + kCrossTile - 1) / kCrossTile;
-    const int j0 = (int)((int64_t)all * split / p.splits), n = (int)((int64_t)all * (split + 1) / p.splits) - j0;      // the block's tiles of tokens
+    // The block's tiles of tokens (2^23 at most in all, and no more cuts than SMs: 32 bits).
+    const int j0 = (int)((uint32_t)all * (uint32_t)split / (uint32_t)s.cuts), n = (int)((uint32_t)all * (uint32_t)(split + 1) / (uint32_t)s.cuts) - j0;
     if (LAID && tid == 9 * 32 && n > 0) {             // the matrix of the way in, see below
         split_expect(raw_full, kCrossImage);
         cross_copy(M::kWay, p.turn_image + kCrossImage, kCrossImage, raw_full);
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 turn ^= 1;
             }
         }
-        if (on_k && ok && n > 0 && p.splits == 1) {
+        if (on_k && ok && n > 0 && cut_over() == 1) {
             // =============================== the matrix of the way back ======================================
             const int item = k_item(n), slot = item % M::kImages;
             ok = cross_wait(img_empty + 8 * slot, ((item / M::kImages) & 1) ^ 1, gone) && (item != M::kImages - 1 || cross_wait(turned, 0, gone));
@@ -733,11 +742,11 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (LAID && warp == 8) {
             // =============================== copies: images ===============================================
-            const int items = n == 0 ? 0 : solo || p.splits == 1 ? 2 * n + 1 : 2 * n;
+            const int items = n == 0 ? 0 : solo || cut_over() == 1 ? 2 * n + 1 : 2 * n;
             int k = 0;
             for (; k < items; k++) {
                 const int slot = k % M::kImages, v = solo ? k > 0 && !(k & 1) : k & 1, t = solo ? v ? (k >> 1) - 1 : (k + 1) >> 1 : k >> 1;      // item k is V (t) or K (t)
-                if (t == n && p.splits > 1) continue;
+                if (t == n && cut_over() > 1) continue;
                 if (!cross_wait(img_empty + 8 * slot, ((k / M::kImages) & 1) ^ 1, gone) || (k == M::kImages - 1 && !cross_wait(turned, 0, gone))) break;
                 if (lane == 0) {
                     const uint8_t* const from = t == n ? p.turn_image : p.kv_images + (((int64_t)(s.kv0 + j0 + t) * H + h) * 2 + v) * kCrossImage;
@@ -956,7 +965,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                     __syncwarp();
                 }
             }
-            if (ok && p.splits == 1) {                // the way back: two parts of O's rows, in S's place, against the matrix in V's; of one tile, both groups' O
+            if (ok && cut_over() == 1) {              // the way back: two parts of O's rows, in S's place, against the matrix in V's; of one tile, both groups' O
                 ok = image_there(k_item(n), 1);
                 for (int i = 0; i < (solo && n == 1 ? 1 : 2) && ok; i++) {
                     ok = cross_wait(a_full + 8 * i, 0, gone);
@@ -1208,7 +1217,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         tc_fence_after();
         // O of the row is in units of 2^ev_ref; one tile's two groups bring theirs to the larger.  (What is written to the queries' place: by now all S are formed.)
         float scale = 1.0f;
-        const bool cut = p.splits > 1;
+        const bool cut = cut_over() > 1;
         if (solo && n > 0 && !cut) {
             float4* const sums = reinterpret_cast<float4*>(window + M::kQ);
             sums[tid] = make_float4(m, l, ev_ref, 0.0f);
@@ -1344,17 +1353,22 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
     grid_launch_dependents();
     grid_dependency_wait();
     if (at >= rows) return;
-    const int parts = 2 * p.splits;
-    float lse = lane < parts ? p.partial_lse[lane * rows + at] : -INFINITY;      // of the first 32 parts, a lane each
-    // a row that belongs to no sequence, or to one that was left out, is left as it is
+    float lse = lane < 2 * p.splits ? p.partial_lse[lane * rows + at] : -INFINITY;      // of the first 32 parts, a lane each; fewer count, see below
+    // a row that belongs to no sequence, to one that was left out or to one that a single block takes is left as it is
     const int t = (int)(at / p.f.real_heads);
-    bool live = false;
-    for (int base = 0; base < p.f.batch && !live; base += 32) {
+    int cuts = 1;
+    for (int base = 0; base < p.f.batch; base += 32) {
         bool bad;
         const bool in = base + lane < p.f.batch && cross_qlen(p, base + lane, bad) > 0 && p.cu_q[base + lane] <= t && t < p.cu_q[base + lane + 1];
-        live = __any_sync(0xffffffffu, in);
+        const uint32_t where = __ballot_sync(0xffffffffu, in);
+        if (where) {
+            cuts = cross_cuts(p, cross_len(p, base + __ffs(where) - 1, bad));
+            break;
+        }
     }
-    if (!live) return;
+    if (cuts == 1) return;
+    const int parts = 2 * cuts;
+    if (lane >= parts) lse = -INFINITY;
     float m = lse, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 32 + lane; s < parts; s += 32) m = fmaxf(m, p.partial_lse[s * rows + at]);
 #pragma unroll
@@ -1409,7 +1423,7 @@ static CrossLayout cross_layout(int batch, int total_q, int64_t total_tokens, in
     l.items = rows / per + batch;                           // every sequence may end inside one
     l.kv_room = total_tokens / kCrossTile + batch;
     l.laid = rows > (int64_t)kCrossLaid * kCrossTile * batch;
-    // As many cuts of the tokens as fill the SMs, of two tiles (one a warpgroup) at least.
+    // As many cuts of the longest sequence's tokens as fill the SMs, of two tiles (one a warpgroup) at least; see cross_cuts.
     const int64_t some = (rows + per - 1) / per, blocks = (some > batch ? some : batch) * kv_heads;
     const int64_t longest = (int64_t)max_pages * kPageTokens < total_tokens ? (int64_t)max_pages * kPageTokens : total_tokens;
     const int64_t most = (longest + 2 * kCrossTile - 1) / (2 * kCrossTile), fit = sms / blocks;
