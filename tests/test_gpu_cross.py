@@ -302,6 +302,39 @@ def test_out_of_range_is_left_out_and_counted():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows_each, lens", [(10, 40), (150, 200), (40, 5000)])
+def test_rows_that_two_ranges_name_belong_to_the_first(rows_each, lens):
+    """A range that goes back in front of the end of an earlier one counts as none, and takes nothing from the others (40 sequences: more than a warp looks at in a step)."""
+    B = 40
+    cache, table, lens_t = paged([lens if b < 34 else 3 for b in range(B)], 1, 128, 4)
+    cu = torch.arange(B + 1, dtype=torch.int32) * rows_each
+    for b in (5, 6, 7, 20, 33):
+        cu[b] = 0                                          # ranges b - 1 fall, ranges b go over rows of others
+    total = B * rows_each
+    lens_t[20] = 0
+    q = torch.randn(total, 2, 128, generator=torch.Generator().manual_seed(0)).half()
+    attn, args = TurboQuantPagedAttention(2, 128, 0.1, 1), (cache.to(DEV), table.to(DEV), lens_t.to(DEV), int(lens_t.sum()))
+    end, whole, faults, clean = 0, [], 0, torch.arange(B + 1, dtype=torch.int32) * rows_each
+    for b in range(B):
+        a, z = int(cu[b]), int(cu[b + 1])
+        if 0 <= a <= z <= total and (a >= end or a == z):      # (no rows: no fault)
+            whole += [b] if z > a else []
+        else:
+            faults += 1
+        end = max(end, z) if 0 <= a < z <= total else end
+    assert whole[-1] == B - 1 and faults > 5
+    good = attn.cross(q.to(DEV), clean.to(DEV), *args).cpu()
+    before = _cabi.state_fault_counts()[0]
+    out, lse = torch.full(q.shape, 9.0, dtype=torch.half, device=DEV), torch.full((total, 2), 9.0, device=DEV)
+    attn.cross(q.to(DEV), cu.to(DEV), *args, out, lse)
+    out, want = out.cpu(), torch.full(q.shape, 9.0, dtype=torch.half)
+    for b in whole:
+        want[b * rows_each:(b + 1) * rows_each] = good[b * rows_each:(b + 1) * rows_each]
+    assert torch.equal(out, want) and _cabi.state_fault_counts()[0] - before == faults
+    assert torch.equal(lse.cpu() == 9, (want == 9).all(-1))
+
+
+@pytest.mark.gpu
 def test_graphs_and_streams():
     """Two captured calls (one cut over blocks, one not), replayed in turn beside eager ones on another stream."""
     runs = []

@@ -90,11 +90,48 @@ __device__ __forceinline__ int cross_len(const CrossParams& p, int b, bool& bad)
     bad = len < 0 || len > (int64_t)p.f.max_pages * kPageTokens;
     return bad ? 0 : len;
 }
-__device__ __forceinline__ int cross_qlen(const CrossParams& p, int b, bool& bad) {
-    const int c0 = p.cu_q[b], c1 = p.cu_q[b + 1];
-    bad = c0 < 0 || c1 < c0 || c1 > p.total_q;
-    return bad ? 0 : c1 - c0;
-}
+// Query rows of N times 32 sequences, a lane each, from their bounds.  A range that is none has no rows, and none has one that begins before the end of an earlier one,
+// which takes bounds that fall somewhere: only from there on the ends are looked at.  A whole warp, one batch of sequences behind the other.
+struct CrossRanges {
+    int end = 0;                // of the ranges so far: the lane's, and once bounds have fallen all lanes'
+    bool fell = false;
+    template <int N>
+    __device__ __forceinline__ void rows(const CrossParams& p, const int (&c0)[N], const int (&c1)[N], int lane, int (&rows)[N], int& faults) {
+        bool falls = false;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const bool bad = c0[e] < 0 || c1[e] < c0[e] || c1[e] > p.total_q;
+            rows[e] = bad ? 0 : c1[e] - c0[e];
+            faults += bad;
+            falls |= c1[e] < c0[e];
+        }
+        if (!fell && __any_sync(0xffffffffu, falls)) {
+            fell = true;
+            end = __reduce_max_sync(0xffffffffu, end);
+        }
+        if (!fell) {
+#pragma unroll
+            for (int e = 0; e < N; e++) end = max(end, rows[e] > 0 ? c1[e] : 0);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const int upto = rows[e] > 0 ? c1[e] : 0;
+            int before = __shfl_up_sync(0xffffffffu, upto, 1);
+            before = lane == 0 ? end : max(before, end);
+#pragma unroll 1
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before = max(before, t);
+            }
+            if (rows[e] > 0 && c0[e] < before) {
+                rows[e] = 0;
+                faults++;
+            }
+            end = max(end, __reduce_max_sync(0xffffffffu, upto));
+        }
+    }
+};
 // Blocks that a sequence's tokens are cut over: two tiles each (one a warpgroup) at least.  By its own length: results depend neither on the table's width nor on
 // the tokens that the caller makes room for, and no block beside these has work (or a partial).
 __device__ __forceinline__ int cross_cuts(const CrossParams& p, int len) { return max(1, min(p.splits, (len + 2 * kCrossTile - 1) / (2 * kCrossTile))); }
@@ -112,15 +149,18 @@ template <int KIND>
 __device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, int lane, CrossSeq& s) {
     constexpr int kAhead = 4;                         // 32 sequences each, whose numbers are on their way together
     int64_t kv = 0, items = 0;
+    CrossRanges ranges;
     for (int base = 0; base < p.f.batch; base += 32 * kAhead) {
-        int len[kAhead], qlen[kAhead];
+        int len[kAhead], qlen[kAhead], c0[kAhead], c1[kAhead], faults = 0;
 #pragma unroll
         for (int e = 0; e < kAhead; e++) {
             const int b = base + 32 * e + lane;
             bool bad;
             len[e] = b < p.f.batch ? cross_len(p, b, bad) : 0;
-            qlen[e] = b < p.f.batch ? cross_qlen(p, b, bad) : 0;
+            c0[e] = b < p.f.batch ? p.cu_q[b] : 0;
+            c1[e] = b < p.f.batch ? p.cu_q[b + 1] : 0;
         }
+        ranges.rows(p, c0, c1, lane, qlen, faults);
         bool hit = false;
         int kt = 0, mine = 0;
 #pragma unroll
@@ -156,11 +196,15 @@ __device__ __forceinline__ bool cross_find(const CrossParams& p, int64_t index, 
 __device__ __forceinline__ void cross_count_faults(const CrossParams& p, int lane) {
     int64_t kv = 0;
     int faults = 0;
+    CrossRanges ranges;
     for (int base = 0; base < p.f.batch; base += 32) {
-        bool bad_len = false, bad_q = false;
-        const int b = base + lane, len = b < p.f.batch ? cross_len(p, b, bad_len) : 0, qlen = b < p.f.batch ? cross_qlen(p, b, bad_q) : 0;
-        const int kt = qlen > 0 ? (len + kCrossTile - 1) / kCrossTile : 0, to = cross_upto(kt, lane);
-        faults += bad_len + bad_q + (kt > 0 && kv + to > p.kv_room);
+        bool bad_len = false;
+        const int b = base + lane, len = b < p.f.batch ? cross_len(p, b, bad_len) : 0;
+        const int c0[1] = {b < p.f.batch ? p.cu_q[b] : 0}, c1[1] = {b < p.f.batch ? p.cu_q[b + 1] : 0};
+        int qlen[1];
+        ranges.rows(p, c0, c1, lane, qlen, faults);
+        const int kt = qlen[0] > 0 ? (len + kCrossTile - 1) / kCrossTile : 0, to = cross_upto(kt, lane);
+        faults += bad_len + (kt > 0 && kv + to > p.kv_room);
         kv += __shfl_sync(0xffffffffu, to, 31);
     }
     if (faults) atomicAdd(&g_cross_faults, faults);
@@ -222,8 +266,9 @@ __device__ __forceinline__ uint4 cross_way_in(int col, int c, uint32_t negative,
 // images laid out ahead
 // ---------------------------------------------------------------------------------------------
 constexpr int kLayThreads = 256, kLayPitch = 17;      // words of a staged V row (16 and one, for the banks)
+// (Registers for three blocks an SM: left to itself the compiler takes 48, and 8 x 512 fp16 queries on 1500 tokens 238 us in place of 230.)
 template <bool EXACT>
-__global__ void __launch_bounds__(kLayThreads) cross_lay_out_kernel(const __grid_constant__ CrossParams p) {
+__global__ void __launch_bounds__(kLayThreads, 3) cross_lay_out_kernel(const __grid_constant__ CrossParams p) {
     __shared__ uint32_t lut[256 * 32];                // entry v, column lane: {level(v & 15), level(v >> 4)}
     __shared__ uint32_t codes_s[kCrossTile * kLayPitch];
     __shared__ int64_t slot_s[kCrossTile];            // byte of each token's K slot
@@ -1357,11 +1402,14 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const __grid_constant__
     // a row that belongs to no sequence, to one that was left out or to one that a single block takes is left as it is
     const int t = (int)(at / p.f.real_heads);
     int cuts = 1;
+    CrossRanges ranges;
     for (int base = 0; base < p.f.batch; base += 32) {
-        bool bad;
-        const bool in = base + lane < p.f.batch && cross_qlen(p, base + lane, bad) > 0 && p.cu_q[base + lane] <= t && t < p.cu_q[base + lane + 1];
-        const uint32_t where = __ballot_sync(0xffffffffu, in);
+        const int b = base + lane, c0[1] = {b < p.f.batch ? p.cu_q[b] : 0}, c1[1] = {b < p.f.batch ? p.cu_q[b + 1] : 0};
+        int qlen[1], faults = 0;
+        ranges.rows(p, c0, c1, lane, qlen, faults);
+        const uint32_t where = __ballot_sync(0xffffffffu, qlen[0] > 0 && c0[0] <= t && t < c1[0]);
         if (where) {
+            bool bad;
             cuts = cross_cuts(p, cross_len(p, base + __ffs(where) - 1, bad));
             break;
         }
