@@ -223,6 +223,43 @@ def test_tiles_of_different_norms():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("where", [0, 128, 1280])
+@pytest.mark.parametrize("batch, queries, n", [(100, 8, 1500), (2, 2000, 3000), (1, 3, 100000)])
+def test_small_values_that_have_the_weight(batch, queries, n, where, dtype):
+    """The weight lies on two tokens of one tile, whose values are 2^-24 of those of the other tiles.  These weigh less than e^-16 in all, at most about as much in the row: it is as
+    exact as any other, whether they come before or behind."""
+    D = 128
+
+    def norms(rng, shape):
+        x = np.full(shape, 8.0)
+        x[1] = 2.0 ** 13
+        return x
+    cache, table, _ = paged([n], 1, D, 3, norms=norms)
+    at, other = where + 50, where + 77
+    slots = cache.view(2, -1, 1, 80)
+    tile = [int(table[0, t // PAGE]) * PAGE + t % PAGE for t in range(where, where + 128)]
+    slots[1, tile, 0, 64:66] = torch.from_numpy(np.frombuffer(np.float16(2.0 ** -11).tobytes(), np.uint8).copy())
+    k, v = rows(cache, table[0], n, D)
+    gen = np.random.default_rng(5)
+    a, c = (k[t, 0] / np.linalg.norm(k[t, 0]) for t in (at, other))
+    q = 6.0 * (a + c) * (1 + 0.02 * gen.standard_normal((batch * queries, 2, 1))) + 0.02 * (a - c) * gen.standard_normal((batch * queries, 2, 1))
+    q = torch.from_numpy(q).to(dtype)
+    o, _, w, _ = attend(q.double().numpy(), k, v, 1.0)
+    assert (np.delete(w, [at, other], -1).sum(-1) < np.exp(-16.0)).all()
+    attn = TurboQuantPagedAttention(2, D, 1.0, 1)
+    out = attn.cross(q.to(DEV), (torch.arange(batch + 1, dtype=torch.int32) * queries).to(DEV), cache.to(DEV), table.expand(batch, -1).to(DEV),
+                     torch.full((batch,), n, dtype=torch.int32, device=DEV), batch * n, torch.empty(q.shape, device=DEV) if dtype == torch.float16 else None)
+    # As above, of these weights; P below 2^-14 is rounded within 2^-25 of the row's largest w |v|.
+    dx = (2.0 ** -13 + 2.0 ** -17 + (2.0 ** -10 if dtype == torch.bfloat16 else 0)) * np.linalg.norm(q.double().numpy(), axis=-1) * 8 * 1.002
+    share = w * np.linalg.norm(v[:, 0], axis=-1)
+    tol = share.sum(-1) * (2.0 ** -11 + 2.0 ** -13 + (2.0 ** -11 + half_step(dtype) if dtype == torch.bfloat16 else 2.0 ** -24) + 2 * dx + 2.0 ** -19)
+    tol += n * 2.0 ** -25 * share.max(-1)
+    d = np.linalg.norm(out.cpu().double().numpy() - o, axis=-1)
+    assert (d <= tol).all(), (d / tol).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_nan_and_infinite_queries_reach_their_rows_alone(dtype):
     cache, table, lens = paged([300, 200], 2, 128, 4)
     q = torch.randn(200, 8, 128, generator=torch.Generator().manual_seed(0)).to(dtype)

@@ -20,8 +20,8 @@
 //
 // S, then P, and O of two tiles are all of tensor memory: 2 x (128 + 128) columns.  With two tiles of query rows each warpgroup has one, and while it works out
 // exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn; at the end each brings its O to the
-// larger of their maxima, and the product that rotates back adds them.  The running maximum is raised only when a logit exceeds it by 2^8, which makes
-// rescaling O rare; a row needs no other thread but its own.  Where few rows have long sequences the tokens are cut over several blocks as well: every group
+// larger of their maxima, and the product that rotates back adds them.  The running maximum, of the logit and the logarithm of V's scale in its tile together, is raised
+// only when one exceeds it by 2^8, which makes rescaling O rare; a row needs no other thread but its own.  Where few rows have long sequences the tokens are cut over several blocks as well: every group
 // leaves a partial, and a second kernel joins them.
 //
 // The rotations are matrix products too, with a matrix of ones and minus ones, exact in any type: the queries go through the tensor core as they come before the
@@ -35,7 +35,8 @@
 // thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 20.7 us, two tiles a block.
 //
 // Numbers are fp16 in the tensor core with fp32 sums, brought into fp16's range by powers of two: a query row by its largest element, the norms of
-// K and V by the largest of the tile.
+// K and V by the largest of the tile, P by the largest share that a tile can have in the row.  (By the largest weight alone, tiles whose values are small beside those of
+// earlier tiles kept few bits, even where they had all the weight: values 2^-24 of the others' none.)
 //   16-bit results of 8 bits (bf16): norms are multiplied into K^ and V^, one rounding (2^-12) each.
 //   results of 11 bits and more (fp16, fp32): K^ and V^ are bare levels, scaled so that the eight of them lie within 4e-5 of fp16 values;
 //             norms multiply S and P in fp32, and a query is two fp16 parts (half again as many operations in the tensor core, and one
@@ -58,7 +59,7 @@ constexpr int kCrossRowThreads = 384, kCrossThreads = kCrossRowThreads + 2 * kCr
 constexpr int kCrossLaid = 2;
 constexpr float kCrossRaise = 8.0f;                  // P up to 2^8
 constexpr double kCrossLevelScale = 1.42803;         // see tq_scored.cu
-constexpr float kCrossNoNorm = -1000.0f;             // the logarithm of V's scale in a tile whose V is all zero
+constexpr float kCrossNoNorm = -40.0f;               // the logarithm of V's scale in a tile whose V is all zero: below that of any other
 constexpr uint32_t kCrossWaitLimit = 1u << 18, kCrossSuspendNs = 1000;
 
 struct CrossParams {
@@ -226,8 +227,8 @@ __device__ __forceinline__ int cross_exponent(float v, int to) {
 }
 __device__ __forceinline__ float cross_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// Where the largest norm of a tile goes, as an exponent of two.  In the images: products with levels up to 4 stay inside fp16.  Under P (exact): P is up to 2^9, and
-// an earlier tile's scale may be 2^6 behind.
+// Where the largest norm of a tile goes, as an exponent of two.  In the images: products with levels up to 4 stay inside fp16.  Under P (exact): below one, so that P
+// times a norm is no larger than P.
 constexpr int kCrossInImage = 6, kCrossUnderP = -1;
 
 // Piece c (eight columns) of row dim of the matrix of the way back: column 16 d + w is dim 8 w + d of O.
@@ -1121,7 +1122,9 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             asm volatile("bar.sync 2, 288;" ::: "memory");
             if (!ok) *gone = 1;
         }
-        float m = kNoMax, l = 0.0f, ev_ref = kCrossNoNorm;
+        // P is taken relative to 2^m, m the running maximum of (logit + ev), 2^ev the scale of the tile's V: a token's share of the row, not its weight alone, decides
+        // how many bits of it are left.  l is the sum of the weights, s that of P, both in units of 2^m; |O| is below s times the largest entry of V's image.
+        float m = kNoMax, l = 0.0f, s_p = 0.0f;
         const int turns = solo ? (n + 1 - i) >> 1 : n;
         for (int k = 0; k < turns && ok; k++) {
             const int t = solo ? 2 * k + i : k;
@@ -1134,10 +1137,8 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             const float kf = fmaxf(scales.x * q_scale, 1e-36f), ev = scales.y;
             const int valid = s.len - (j0 + t) * kCrossTile;
             const P2 kf2 = pk(kf, kf);
-            // P is scaled by 2^dv: a tile whose V is zero, or as good as that beside others, by 2^-60, out of fp16 but not out of the row's sum.  Where the norms
-            // multiply P as they are, dv is that of the sums alone.
-            auto shift = [&] { return EXACT ? fminf(fmaxf(-ev_ref, -60.0f), 60.0f) : fmaxf(ev - ev_ref, -60.0f); };
-            float dv = shift();
+            // Where the norms multiply P as they are (exact) it is the weight that comes from the exponential, else P.
+            const float weight = EXACT ? 1.0f : cross_power(-(int)ev), share = EXACT ? cross_power((int)ev) : 1.0f;      // of one of its sum
             // Norms of eight tokens, fp16 as in the cache (a broadcast load costs a wavefront for every four bytes: half of what fp32 ones would).
             auto times_norms = [&](int which, int col, float* v) {
                 const uint4 a = lds128(norms + 2 * (kCrossTile * which + col));
@@ -1168,9 +1169,9 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             bool done = false;
             // In the common case the running maximum needs no look at the row: P is worked out from the maximum that there is, and its sum tells whether any of it
             // is too large (2^9; NaN and infinity too).  P waits in registers until the warp knows, as it takes the place of S.
-            if (valid >= kCrossTile && ev <= ev_ref + 6.0f) {
-                const P2 sub = pk(dv - m, dv - m);
-                const float most = 512.0f * fast_exp2(dv);
+            if (k > 0 && valid >= kCrossTile) {
+                const float from = EXACT ? -m : ev - m;
+                const P2 sub = pk(from, from);
                 uint32_t ph[64];
                 float v[2][16];                       // the next columns are on their way
                 cross_ld16(tm_s, v[0]);
@@ -1186,7 +1187,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 }
                 float sa, sb;
                 up(sum, sa, sb);
-                done = __all_sync(0xffffffffu, sa + sb <= most);
+                done = __all_sync(0xffffffffu, (sa + sb) * share <= 512.0f);
                 if (done) {
                     cross_st(tm_s, ph);
                     cross_st(tm_s + 32, ph + 32);
@@ -1214,17 +1215,13 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
 #pragma unroll
                     for (int e = 0; e < 32; e++) top = fmaxf(top, v[e]);
                 }
-                top *= kf;                            // kf > 0
+                top = top * kf + ev;                  // kf > 0
                 const bool raise = top > m + kCrossRaise;
-                // The power of two of V that the sums are kept in is the first tile's, until a tile's is 2^6 above it.
-                if (__any_sync(0xffffffffu, raise) || ev > ev_ref + 6.0f) {
-                    float c = raise ? fast_exp2(m - top) : 1.0f;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float c = raise ? fast_exp2(m - top) : 1.0f;
                     if (raise) m = top;
                     l *= c;
-                    if (ev > ev_ref + 6.0f) {
-                        c *= fast_exp2(ev_ref - ev);
-                        ev_ref = ev;
-                    }
+                    s_p *= c;
                     if (k > 0) {                      // S is there, so the products before it are done with O
 #pragma unroll 1
                         for (int a = 0; a < 4; a++) {
@@ -1236,8 +1233,8 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                         }
                     }
                 }
-                dv = shift();
-                const P2 sub = pk(dv - m, dv - m);
+                const float from = EXACT ? -m : ev - m;
+                const P2 sub = pk(from, from);
                 sum = pk(0.0f, 0.0f);
 #pragma unroll 1
                 for (int c = 0; c < 4; c++) {
@@ -1250,7 +1247,8 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             }
             float sa, sb;
             up(sum, sa, sb);
-            l += (sa + sb) * fast_exp2(-dv);
+            l += (sa + sb) * weight;
+            s_p += (sa + sb) * share;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -1260,24 +1258,25 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
         if (ok && n > 0) ok = cross_wait(o_full + 8 * (turns > 0 ? i : 0), 0, gone);
         if (!ok) *gone = 1;
         tc_fence_after();
-        // O of the row is in units of 2^ev_ref; one tile's two groups bring theirs to the larger.  (What is written to the queries' place: by now all S are formed.)
+        // One tile's two groups bring their sums to the larger of their maxima.  (What is written to the queries' place: by now all S are formed.)
         float scale = 1.0f;
         const bool cut = cut_over() > 1;
         if (solo && n > 0 && !cut) {
             float4* const sums = reinterpret_cast<float4*>(window + M::kQ);
-            sums[tid] = make_float4(m, l, ev_ref, 0.0f);
+            sums[tid] = make_float4(m, l, s_p, 0.0f);
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float4 other = sums[tid ^ 128];
-            const float mm = fmaxf(m, other.x), ev = fmaxf(ev_ref, other.z), c0 = fast_exp2(m - mm);
-            scale = c0 * fast_exp2(ev_ref - ev);
-            l = l * c0 + other.y * fast_exp2(other.x - mm);
+            const float mm = fmaxf(m, other.x), c1 = fast_exp2(other.x - mm);
+            scale = fast_exp2(m - mm);
+            l = l * scale + other.y * c1;
+            s_p = s_p * scale + other.z * c1;
             m = mm;
-            ev_ref = ev;
             if (*gone) ok = false;
         }
         if (__all_sync(0xffffffffu, ok)) {
             const bool none = l == 0.0f, live = row < rows;
-            const float unit = p.f.v_scale * fast_exp2(ev_ref);
+            const int by = cross_exponent(s_p, EXACT ? 12 : 5);
+            const float to_parts = cross_power(by);
             const int qi = row / G, g = row - qi * G;
             const int64_t to = live ? (int64_t)(q_first + qi) * p.f.real_heads + h * G + g : -1;
             const float lse2 = none ? -INFINITY : m + log2f(l);
@@ -1288,7 +1287,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                     p.partial_lse[at] = lse2;
                     if (!solo) p.partial_lse[at + part] = -INFINITY;
                 }
-                scale = unit / l;
+                scale = p.f.v_scale / l;
 #pragma unroll 1
                 for (int c = 0; c < 4 && turns > 0; c++) {
                     float v[32];
@@ -1302,9 +1301,8 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 }
             }
             if (turns > 0 && !cut) {
-                // The weighted mean as two fp16 parts in S's place (at most 2^15: a mean of rows of levels below 4 times norms below 2^7, under powers of two up to
-                // 2^6).
-                scale *= none ? 0.0f : 1.0f / l;
+                // O as two fp16 parts in S's place, by a power of two to below 2^15: the images have levels below 4, in the one form times norms below 2^7.
+                scale *= to_parts;
 #pragma unroll 1
                 for (int c = 0; c < 4; c++) {
                     float v[32];
@@ -1347,7 +1345,7 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
                 }
             };
             const bool whole = p.f.out_dtype != TQ_F32 && D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f.out) & 15) == 0;
-            const float f = unit * p.f.scale;
+            const float f = p.f.v_scale * p.f.scale * cross_power(-by) * (1.0f / l);
 #pragma unroll 1
             for (int c = solo ? 2 * i : 0; c < (solo ? 2 * i + 2 : 4) && ok && !cut; c++) {
                 float v[32];
