@@ -13,7 +13,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.cache_ref import PAGE, attend, half_step, paged, rows
+from tests import cache_rounded
+from tests.cache_ref import LEVELS, PAGE, attend, half_step, paged, rows
 from turboquant_b200 import TurboQuantPagedAttention, _cabi
 
 DEV = "cuda"
@@ -90,6 +91,59 @@ def test_refusals_of_the_library():
     assert call(d=64)[0] == 2 and call(d=129)[0] == 2 and call(bs=32)[0] == 2 and call(slot=144)[0] == 2
     assert call(hq=9)[0] == 1 and call(cache=None)[0] == 1 and call(qt=-1)[0] == 1 and call(ot=3)[0] == 1 and call(pages=0)[0] == 1 and call(tokens=-1)[0] == 1
     assert call(nb=0)[0] == 1 and call(cache=ctypes.c_void_p(4104))[0] == 1 and call(signs=ctypes.c_void_p(4100))[0] == 1
+
+
+# ---- errors of ordinary rows ------------------------------------------------------------------------
+# The bounds above are for the worst row; that of N(0, 1) rows as a whole is told apart from its nearest mistakes by what the roundings of the operands alone leave
+# (tests/cache_rounded.py): the kernel's error is at most 5/4 of it, and 2^-16 (outputs), 2^-17 (lse) for 32-bit sums, whose steps cut off at 2^-24 of what
+# they add to.  A bf16 result has a uniform error of its own, a step over sqrt(12), 2^-7 of an element at most.
+ORDINARY = [(24, 1500), (600, 1029), (16, 20000), (600, 5000)]          # looked up and laid out, whole and cut
+
+
+def ordinary(queries, n, dtype):
+    cache, table, lens = paged([n], 2, 128, 1)
+    q = (2.0 * torch.randn(queries, 4, 128, generator=torch.Generator().manual_seed(1))).to(dtype)
+    code, norm = cache_rounded.states(cache, table[0], n, 128)
+    turned, scale = cache_rounded.turned(q.double().numpy(), 128), 1 / math.sqrt(128)
+    exact = cache_rounded.attend(turned, code, norm, scale, LEVELS, LEVELS, parts=0, p_bits16=False)
+
+    def errors(**mistake):
+        a = dict(levels=cache_rounded.ONE, value_levels=cache_rounded.ONE, parts=1 if dtype == torch.bfloat16 else 2, norms_inside=dtype == torch.bfloat16)
+        out, lse, _ = cache_rounded.attend(turned, code, norm, scale, **{**a, **mistake})
+        return cache_rounded.rms(out - exact[0]) / cache_rounded.rms(exact[0]), cache_rounded.rms(lse - exact[1])
+    out, lse = errors()
+    bounds = math.hypot(1.25 * out, 2.0 ** -7 / math.sqrt(12) if dtype == torch.bfloat16 else 0) + 2.0 ** -16, 1.25 * lse + 2.0 ** -17
+    return (cache, table, lens, q), exact, errors, bounds
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries, n", [(24, 1500), (16, 20000)])
+def test_the_bounds_of_ordinary_rows_tell_mistakes_apart(queries, n, dtype):
+    _, _, errors, (out, lse) = ordinary(queries, n, dtype)
+    cut = n // 256 // 2 * 256
+    mistakes = [dict(left_out=range(t, t + PAGE)) for t in (112, cut, n - n % PAGE - PAGE)]
+    mistakes += [dict(levels=cache_rounded.f16(LEVELS))]                # the levels as they are, unscaled
+    if dtype != torch.bfloat16:
+        mistakes += [dict(parts=1), dict(value_levels=cache_rounded.f16(LEVELS))]
+    if dtype != torch.bfloat16 or n < 2000:                             # (one token of 20000 weighs less than the roundings of a bf16 result)
+        mistakes += [dict(left_out=[t]) for t in (0, 127, 128, cut - 1, cut, n - 1)]
+    for m in mistakes:
+        o, s = errors(**m)
+        assert o > out or s > lse, (m, o, out, s, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries, n", ORDINARY)
+def test_errors_of_ordinary_rows(queries, n, dtype):
+    (cache, table, lens, q), exact, _, bounds = ordinary(queries, n, dtype)
+    out = torch.empty(q.shape, dtype=torch.bfloat16 if dtype == torch.bfloat16 else torch.float32, device=DEV)
+    lse = torch.empty(queries, 4, device=DEV)
+    TurboQuantPagedAttention(4, 128, 1 / math.sqrt(128), 2).cross(q.to(DEV), torch.tensor([0, queries], dtype=torch.int32, device=DEV), cache.to(DEV), table.to(DEV), lens.to(DEV),
+                                                                  n, out, lse)
+    got = cache_rounded.turned(out.cpu().double().numpy(), 128)         # (the way back is no rounding in 64 bits)
+    errors = cache_rounded.rms(got - exact[0]) / cache_rounded.rms(exact[0]), cache_rounded.rms(lse.cpu().double().numpy() - exact[1])
+    assert errors[0] <= bounds[0] and errors[1] <= bounds[1], (errors, bounds)
 
 
 # ---- on the GPU -----------------------------------------------------------------------------------
