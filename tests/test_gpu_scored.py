@@ -13,7 +13,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.cache_ref import PAGE, attend, half_step, paged, rows
+from tests import cache_rounded
+from tests.cache_ref import LEVELS, PAGE, attend, half_step, paged, rows
 from turboquant_b200 import TurboQuantPagedAttention, _cabi
 
 DEV = "cuda"
@@ -103,6 +104,38 @@ def test_rows_of_scores_that_meet_across_heads_and_sequences_are_refused(batch_s
     rc = L.tq_decode_scored(P, I(1), I(2), I(8), I(4), I(128), P, Q(4), I(16), I(80), P, I(2), P, P, ctypes.c_float(0.1), P, Q(batch_stride), Q(head_stride), I(32), I(1),
                             P, ctypes.c_size_t(0), P, I(1), None, None)
     assert rc == 1 and "rows of scores overlap" in L.tq_last_error().decode()
+
+
+# ---- errors of ordinary scores -----------------------------------------------------------------------
+# The bounds above are for the worst score.  Logits of N(0, 1) rows are up to 16 in size (base 2); a step of their sums cuts off at 2^-22 of that, and sixteen steps that go either way
+# come to 4 * 2^-18 = 2^-16.  Relative to a score, as a whole, that is the bound; both tables and both parts of a query leave 1e-7 (tests/cache_rounded.py).
+ORDINARY = [([1000] * 4, 8, 2), ([20000], 8, 2), ([3000] * 3, 16, 2), ([333] * 8, 5, 1)]
+
+
+def ordinary(lens, Hq, H):
+    cache, table, lens_t = paged(lens, H, 128, 1)
+    q = (2.0 * torch.randn(len(lens), Hq, 128, generator=torch.Generator().manual_seed(1))).half()
+
+    def scores(**a):
+        out = []
+        for b, n in enumerate(lens):
+            code, norm = cache_rounded.states(cache, table[b], n, 128)
+            _, _, w = cache_rounded.attend(cache_rounded.turned(q[b:b + 1].double().numpy(), 128), code, norm, 1 / math.sqrt(128), value_levels=LEVELS, **a)
+            out.append(w[0].reshape(H, Hq // H, n).sum(1))
+        return out
+    return (cache, table, lens_t, q), scores(levels=LEVELS, parts=0), scores
+
+
+def relative(got, want):
+    return cache_rounded.rms(np.concatenate([((g - w) / w).ravel() for g, w in zip(got, want)]))
+
+
+@pytest.mark.parametrize("lens, Hq, H", ORDINARY)
+def test_the_bound_of_ordinary_scores_tells_mistakes_apart(lens, Hq, H):
+    _, exact, scores = ordinary(lens, Hq, H)
+    assert relative(scores(levels=cache_rounded.TWO, parts=2), exact) < 2.0 ** -22
+    assert relative(scores(levels=cache_rounded.ONE, parts=2), exact) > 2.0 ** -16          # without the second table
+    assert relative(scores(levels=cache_rounded.TWO, parts=1), exact) > 2.0 ** -16          # without the second part of the queries
 
 
 # ---- on the GPU -----------------------------------------------------------------------------------
@@ -293,3 +326,13 @@ def test_pages_that_never_come_leave_the_scores_alone(lens, Hq, H):
     assert not out[~some].any() and (lse.cpu()[~some] == -np.inf).all()
     out = attn.decode_scored(*d, scores, None, lse).cpu()
     check((cache, table, lens_t, q, before), out, scores.cpu().numpy(), lse.cpu().numpy(), scale=0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens, Hq, H", ORDINARY)
+def test_errors_of_ordinary_scores(lens, Hq, H):
+    (cache, table, lens_t, q), exact, _ = ordinary(lens, Hq, H)
+    scores = torch.zeros(len(lens), H, table.shape[1] * PAGE, device=DEV)
+    TurboQuantPagedAttention(Hq, 128, 1 / math.sqrt(128), H).decode_scored(q.to(DEV), cache.to(DEV), table.to(DEV), lens_t.to(DEV), scores)
+    error = relative([s[:, :n] for s, n in zip(scores.cpu().double().numpy(), lens)], exact)
+    assert error <= 2.0 ** -16, error
