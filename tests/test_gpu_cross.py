@@ -393,7 +393,7 @@ def test_out_of_range_is_left_out_and_counted():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows_each, lens", [(10, 40), (150, 200), (40, 5000)])
+@pytest.mark.parametrize("rows_each, lens", [(10, 40), (150, 200), (300, 200), (40, 5000)])
 def test_rows_that_two_ranges_name_belong_to_the_first(rows_each, lens):
     """A range that goes back in front of the end of an earlier one counts as none, and takes nothing from the others (40 sequences: more than a warp looks at in a step)."""
     B = 40

@@ -14,9 +14,9 @@
 //   two warpgroups, a thread a row, take S from tensor memory, keep a running maximum and sum, and put P (fp16) into the same columns.
 //
 // Where many query rows share a sequence's tokens (prompts), a first kernel writes the images of K and V to memory once and a block only copies them in,
-// 32 KB each: the look-ups take longer than the products they feed (453 us looked up, 299 laid out ahead, at four sequences of 1024 queries on 4096
+// 32 KB each: the look-ups take longer than the products they feed (405 us looked up, 305 laid out ahead, at four sequences of 1024 queries on 4096
 // tokens, 32 heads on 8).  With few rows that would write and read 512 bytes for every 80-byte slot, and the slots are looked up as they
-// come (43 us looked up, 53 laid out ahead, with 32 queries).
+// come (36 us looked up, 56 laid out ahead, with 32 queries).
 //
 // S, then P, and O of two tiles are all of tensor memory: 2 x (128 + 128) columns.  With two tiles of query rows each warpgroup has one, and while it works out
 // exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn; at the end each brings its O to the
@@ -53,10 +53,12 @@ constexpr int kCrossTile = 128;                      // tokens, query rows, padd
 constexpr int kCrossImage = kCrossTile * kCrossTile * 2;
 constexpr int kCrossTeam = 4;                        // warps that look up K, and as many for V
 constexpr int kCrossRowThreads = 384, kCrossThreads = kCrossRowThreads + 2 * kCrossTeam * 32;      // two warpgroups of rows, one of copies, norms and products; the teams
-// Tiles of query rows a sequence, on the average, above which the images are laid out ahead.  32 heads on 8, 8 sequences of 1500 tokens and 4 of 4096, bf16 results: 256 rows
-// 59.4 and 65.5 us laid out, 53.2 and 57.3 looked up, 512 rows 59.4 and 81.9, 63.5 and 86.0; fp16: 256 rows 55.3 and 71.6, 51.2 and 67.6, 512 rows 86.0 and 88.0,
-// 94.2 and 102.4.
-constexpr int kCrossLaid = 2;
+// Tiles of query rows a sequence, on the average, above which the images are laid out ahead.  us laid out and looked up, 32 heads on 8, bf16 / fp16 results:
+//   320 rows    16 x 1500 tokens 110 and 95 / 128 and 121, 32 x 700 123 and 114 / 161 and 163
+//   512 rows    8 x 1500 tokens 59 and 51 / 82 and 82, 4 x 4096 85 and 72 / 89 and 91
+//   768 rows    4 x 4096 103 and 106 / 136 and 167;   1200 rows    4 x 32768 1124 and 1418 / 1308 and 1700
+// and of one sequence 800 rows on 1500 tokens 35 and 31 / 39 and 35, 1600 rows on 65536 587 and 706 / 815 and 1148.
+constexpr int kCrossLaid = 4;
 constexpr float kCrossRaise = 8.0f;                  // P up to 2^8
 constexpr double kCrossLevelScale = 1.42803;         // see tq_scored.cu
 constexpr float kCrossNoNorm = -40.0f;               // the logarithm of V's scale in a tile whose V is all zero: below that of any other
