@@ -32,7 +32,7 @@
 // the tensor core busy for two thirds of a tile's 3000 cycles: 4 x 2048 queries on 4096 tokens, 32 heads on 8, 560 us, 980 TFLOP/s.  Few rows, long
 // sequences: the same chain for one tile, half of its exponentials' time the norms' loads and products (fp16 results), and V's look-ups: 2 x 16
 // queries on 65536 tokens, 64 heads on 8, 173 us, 805 GB/s of codes.  Short ones: what a block does before its first tile and behind its last, some 20
-// thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 20.7 us, two tiles a block.
+// thousand cycles: 24 queries on 1500 tokens, 16 heads on 8, 20.1 us, two tiles a block.
 //
 // Numbers are fp16 in the tensor core with fp32 sums, brought into fp16's range by powers of two: a query row by its largest element, the norms of
 // K and V by the largest of the tile, P by the largest share that a tile can have in the row.  (By the largest weight alone, tiles whose values are small beside those of

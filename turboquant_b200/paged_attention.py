@@ -220,8 +220,9 @@ class TurboQuantPagedAttention:
         """Cross attention: any number of query rows a sequence over ALL of its cached tokens, whose number is another (a decoder's prompt over
         an encoder's states).  ``query`` [rows, heads, head_size], head sizes 65 ... 128; row ``cu_seqlens_q[b] + i`` is query i of
         sequence b.  ``total_tokens``, at least the sum of ``seq_lens``, is passed by the caller (no sync).  A sequence without tokens gives
-        zeros; rows behind ``cu_seqlens_q[-1]`` are left as they were.  Scratch comes from torch's allocator at each call; where hundreds of query
-        rows share them the cached tokens as 16-bit rows are part of it (512 bytes a token and KV head).  Single new tokens go to ``decode``, up to 32 query
+        zeros; rows behind ``cu_seqlens_q[-1]`` are left as they were.  The probabilities are fp16 (2^-12) whatever the result's type; the bits depend neither
+        on the table's width nor on ``total_tokens``.  Scratch comes from torch's allocator at each call; above 512 rows a sequence (queries times query heads of a KV head, on the
+        average) the cached tokens as 16-bit rows are part of it (512 bytes a token and KV head).  Single new tokens go to ``decode``, up to 32 query
         columns that share a sequence to ``decode_shared``: they read the codes as they are."""
         done = self._calls.cross(query, cu_seqlens_q, kv_cache, block_table, seq_lens, total_tokens, output, out_lse)
         if done is not None:
