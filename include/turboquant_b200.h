@@ -387,7 +387,8 @@ int tq_nc_write_dropped(int32_t* count);
  * beyond the page table or beyond total_tokens counts as no tokens, a range of cu_seqlens_q that is none, or that begins before the end of an earlier one, as no
  * rows, and a page id outside [0, num_blocks) reads page 0; all are counted (tq_state_fault_counts).  Results have the same bits whatever max_pages and total_tokens
  * (at least the sum) are.  The workspace (tq_cross_workspace_bytes; 256-byte aligned, no initialising) holds partial rows where sequences are cut, and where many query
- * rows share them the cached tokens as 16-bit rows.  Rows of a block whose (bounded) waits ran out are void, and counted too.  The reference attends fresh keys and values only (turboquant/vllm_backend_fused.py:336-369). */
+ * rows share them the cached tokens as 16-bit rows.  Rows of a block whose (bounded) waits ran out are void, and counted too.  The reference attends fresh
+ * keys and values only (turboquant/vllm_backend_fused.py:336-369). */
 size_t tq_cross_workspace_bytes(int batch, int total_q, int64_t total_tokens, int num_q_heads, int num_kv_heads, int max_pages, int out_dtype);
 int tq_cross(const void* q, int q_dtype, int total_q, const int32_t* cu_seqlens_q, int batch, int num_q_heads, int num_kv_heads, int head_dim,
              const void* kv_cache, int64_t num_blocks, int block_size, int slot_bytes, const int32_t* page_table, int max_pages,

@@ -21,8 +21,8 @@
 // S, then P, and O of two tiles are all of tensor memory: 2 x (128 + 128) columns.  With two tiles of query rows each warpgroup has one, and while it works out
 // exponentials the tensor core works for the other.  With one the warpgroups take the tiles of tokens in turn; at the end each brings its O to the
 // larger of their maxima, and the product that rotates back adds them.  The running maximum, of the logit and the logarithm of V's scale in its tile together, is raised
-// only when one exceeds it by 2^8, which makes rescaling O rare; a row needs no other thread but its own.  Where few rows have long sequences the tokens are cut over several blocks as well: every group
-// leaves a partial, and a second kernel joins them.
+// only when one exceeds it by 2^8, which makes rescaling O rare; a row needs no other thread but its own.  Where few rows have long sequences the tokens are cut over
+// several blocks as well: every group leaves a partial, and a second kernel joins them.
 //
 // The rotations are matrix products too, with a matrix of ones and minus ones, exact in any type: the queries go through the tensor core as they come before the
 // first tile, and O, as two fp16 parts, behind the last, which also brings its columns into order.  As butterflies over registers they took as long as ten tiles: code that a
