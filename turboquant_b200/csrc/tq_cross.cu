@@ -1270,8 +1270,9 @@ __global__ void __launch_bounds__(LAID ? kCrossRowThreads : kCrossThreads, 1) cr
             const float4 other = sums[tid ^ 128];
             const float mm = fmaxf(m, other.x), c1 = fast_exp2(other.x - mm);
             scale = fast_exp2(m - mm);
-            l = l * scale + other.y * c1;
-            s_p = s_p * scale + other.z * c1;
+            // (Each product rounded by itself: the two groups have to come to the same bits, as the power of two that their parts are brought to follows from them.)
+            l = __fadd_rn(__fmul_rn(l, scale), __fmul_rn(other.y, c1));
+            s_p = __fadd_rn(__fmul_rn(s_p, scale), __fmul_rn(other.z, c1));
             m = mm;
             if (*gone) ok = false;
         }
