@@ -110,6 +110,19 @@ def test_what_the_debug_checks_find(monkeypatch, change, words):
         _cabi.evict(**{**_meta(seq_lens=torch.tensor([64, 17], dtype=torch.int32)), **change})
 
 
+def test_the_debug_checks_of_an_empty_batch(monkeypatch):
+    """Nothing to find: no kernel is reached, and nothing is raised (cross and the scored decode go through the same checks)."""
+    monkeypatch.setattr(_cabi, "_cuda", lambda t, name: None)
+    monkeypatch.setenv("TQ_DEBUG_CHECKS", "1")
+    none = dict(page_table=torch.zeros(0, 4, dtype=torch.int32), seq_lens=torch.zeros(0, dtype=torch.int32))
+    ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32)
+    _cabi.evict(**_meta(**none, scores=torch.zeros(0, 4, 64), out_scores=torch.zeros(0, 4, 16), out_page_table=ints(0, 1), kept=ints(0, 4, 16), new_lens=ints(0)))
+    cache, signs = torch.zeros(2, 4, PAGE, 2, 80, dtype=torch.uint8), torch.ones(128)
+    q = torch.zeros(0, 8, 128)
+    assert _cabi.decode_scored(q, cache, none["page_table"], none["seq_lens"], signs, 0.1, torch.zeros(0, 2, 64), q) is q
+    assert _cabi.cross(q, ints(1), cache, none["page_table"], none["seq_lens"], 0, signs, 0.1, q) is q
+
+
 @pytest.mark.gpu
 def test_debug_checks_of_the_public_call(monkeypatch):
     """Found on the host ahead of any kernel; what is in order runs as ever."""

@@ -114,11 +114,13 @@ def _check_slots(slot_mapping: torch.Tensor, num_blocks: int, block_size: int) -
 
 def _check_pages(page_indices, page_indptr, max_pages, seq_lens, num_blocks: int, block_size: int) -> None:
     lens = seq_lens.to(torch.int64)
-    if lens.numel() and int(lens.min().item()) < 0:
+    if not lens.numel():
+        return
+    if int(lens.min().item()) < 0:
         raise TurboQuantError("seq_lens holds a negative length")
     need = (lens + block_size - 1) // block_size
     if page_indptr is None:
-        if lens.numel() and int(need.max().item()) > max_pages:
+        if int(need.max().item()) > max_pages:
             raise TurboQuantError(f"a sequence needs {int(need.max().item())} pages but the block table has {max_pages} per row")
         rows = page_indices.reshape(lens.numel(), -1)[:, :max_pages].to(torch.int64)
         used = torch.arange(rows.shape[1], device=rows.device)[None, :] < need[:, None]
