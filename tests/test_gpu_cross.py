@@ -80,6 +80,19 @@ def test_refusals_of_the_python_layer(monkeypatch, change, words):
         _cabi.cross(**_args(**change))
 
 
+@pytest.mark.parametrize("change, words", [
+    (dict(cu_seqlens_q=torch.tensor([0, 3, 2], dtype=torch.int32)), "cu_seqlens_q must go"), (dict(cu_seqlens_q=torch.tensor([-1, 3, 5], dtype=torch.int32)), "cu_seqlens_q must go"),
+    (dict(cu_seqlens_q=torch.tensor([0, 3, 6], dtype=torch.int32)), "cu_seqlens_q must go"), (dict(total_tokens=39), "total_tokens says 39"),
+    (dict(seq_lens=torch.tensor([33, 1], dtype=torch.int32)), "needs 3 pages"), (dict(page_table=torch.full((2, 2), 4, dtype=torch.int32)), "page id out of range"),
+])
+def test_what_the_debug_checks_find(monkeypatch, change, words):
+    monkeypatch.setattr(_cabi, "_cuda", lambda t, name: None)
+    monkeypatch.setenv("TQ_DEBUG_CHECKS", "1")
+    good = dict(cu_seqlens_q=torch.tensor([0, 3, 5], dtype=torch.int32), seq_lens=torch.tensor([30, 10], dtype=torch.int32), total_tokens=40)
+    with pytest.raises(_cabi.TurboQuantError, match=words):
+        _cabi.cross(**_args(**{**good, **change}))
+
+
 def test_refusals_of_the_library():
     import ctypes
     L, P, I, Q = _cabi.lib(), ctypes.c_void_p(4096), ctypes.c_int, ctypes.c_int64

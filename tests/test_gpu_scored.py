@@ -83,6 +83,13 @@ def test_refusals_of_the_python_layer(monkeypatch, change, words):
         _cabi.decode_scored(**_args(**change))
 
 
+def test_the_debug_checks_look_at_the_room_of_the_scores(monkeypatch):
+    monkeypatch.setattr(_cabi, "_cuda", lambda t, name: None)
+    monkeypatch.setenv("TQ_DEBUG_CHECKS", "1")
+    with pytest.raises(_cabi.TurboQuantError, match="room for 31"):
+        _cabi.decode_scored(**_args(seq_lens=torch.tensor([32, 1], dtype=torch.int32), scores=torch.zeros(2, 2, 31)))
+
+
 def test_refusals_of_the_library():
     import ctypes
     L, P, I, Q = _cabi.lib(), ctypes.c_void_p(4096), ctypes.c_int, ctypes.c_int64

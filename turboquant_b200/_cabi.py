@@ -587,6 +587,11 @@ def _scores(scores, name: str, batch: int, heads: int) -> None:
         raise TurboQuantError(f"{name}: the scores of a row must be contiguous")
 
 
+def _check_scores(scores, seq_lens) -> None:
+    if seq_lens.numel() and int(seq_lens.max().item()) > scores.shape[2]:
+        raise TurboQuantError(f"a sequence has {int(seq_lens.max().item())} tokens but its scores have room for {scores.shape[2]}")
+
+
 def _on(device):
     """Makes ``device`` the current one for the launches of a call."""
     return torch.cuda.device(device) if torch.cuda.current_device() != device.index else contextlib.nullcontext()
@@ -621,6 +626,11 @@ def cross(q, cu_seqlens_q, kv_cache, page_table, seq_lens, total_tokens: int, si
         raise TurboQuantError(f"total_tokens must not be negative, got {total_tokens}")
     if debug_checks():
         _check_pages(page_table, None, page_table.shape[1], seq_lens, nb, bs)
+        bounds = cu_seqlens_q.tolist()
+        if bounds[0] < 0 or bounds[-1] > T or bounds != sorted(bounds):
+            raise TurboQuantError(f"cu_seqlens_q must go from 0 or more up to {T} rows or fewer, never back")
+        if int(seq_lens.sum().item()) > total_tokens:
+            raise TurboQuantError(f"the sequences have {int(seq_lens.sum().item())} tokens, total_tokens says {total_tokens}")
     if B == 0 or T == 0:
         return out
     f = lib().tq_cross_workspace_bytes
@@ -654,6 +664,7 @@ def decode_scored(q, kv_cache, page_table, seq_lens, signs, sm_scale: float, sco
         raise TurboQuantError(f"new_tokens must not be negative, got {new_tokens}")
     if debug_checks():
         _check_pages(page_table, None, page_table.shape[1], seq_lens, nb, bs)
+        _check_scores(scores, seq_lens)
     if B == 0:
         return out
     f = lib().tq_decode_scored_workspace_bytes
@@ -690,8 +701,7 @@ def evict(kv_cache, page_table, seq_lens, scores, keep: int, recent: int, out_pa
             raise TurboQuantError("the output table is the page table itself: leave it out to evict within the same pages")
     if debug_checks():
         _check_pages(page_table, None, page_table.shape[1], seq_lens, nb, bs)
-        if B and int(seq_lens.max().item()) > scores.shape[2]:
-            raise TurboQuantError(f"a sequence has {int(seq_lens.max().item())} tokens but its scores have room for {scores.shape[2]}")
+        _check_scores(scores, seq_lens)
         if out_page_table is not None:
             _check_pages(out_page_table, None, out_page_table.shape[1], seq_lens.clamp(max=keep), nb, bs)
     if B == 0:
