@@ -396,3 +396,21 @@ def test_the_largest_keep():
     kept, new_lens = TurboQuantPagedAttention(1, 64, 0.1, 1).evict(d, table.to(DEV), lens.to(DEV), scores.to(DEV), keep, 0, None, torch.zeros(1, 1, 112, device=DEV))
     assert new_lens.tolist() == [100] and torch.equal(d.cpu(), cache) and kept.shape == (1, 1, keep)
     assert kept[0, 0, :100].tolist() == list(range(100)) and int(kept[0, 0, 100:].amin()) == int(kept[0, 0, 100:].amax()) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("lens, keep", [([333, 100, 0], 50), ([9000, 20, 4100], 3000)])
+def test_tables_and_scores_far_wider_than_the_sequences(lens, keep, in_place):
+    """Room for 160000 tokens a row, as engines keep it: what is behind a sequence is not looked at, and the launch that the room asks for gives the same."""
+    cache, table, out_table, lens_t, scores = case(lens, 2, 128, keep, 5)
+    wide = torch.full((len(lens), 10000), -3, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    room = torch.full((len(lens), 2, 160000), float("inf"))
+    for b, n in enumerate(lens):
+        room[b, :, :n] = scores[b, :, :n]
+    want = expected(cache, table, table if in_place else out_table, lens_t, scores, torch.zeros(len(lens), 2, keep), keep, 7)
+    d_cache, out = cache.to(DEV), torch.zeros(len(lens), 2, keep, device=DEV)
+    kept, new_lens = TurboQuantPagedAttention(2, 128, 0.1, 2).evict(d_cache, wide.to(DEV), lens_t.to(DEV), room.to(DEV), keep, 7, None if in_place else out_table.to(DEV), out)
+    for got, w in ((kept, want[0]), (new_lens, want[1]), (d_cache, want[2]), (out, want[3])):
+        np.testing.assert_array_equal(got.cpu().numpy(), w)
